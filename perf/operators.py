@@ -309,27 +309,36 @@ def _key(value, index):
     return ordered * (1 << 32) + ((1 << 32) - 1 - index)
 
 
+def _before(a, b):
+    """Which candidates (total, beam, logit, token) come before which: a larger total; of equal ones the lower beam's, and of
+    one beam's that with the larger logit, then the lower token. [n, count of b, count of a]."""
+    (t, k, x, v), (u, l, y, w) = [[part[:, None, :] for part in a], [part[:, :, None] for part in b]]
+    return (t > u) | ((t == u) & ((k < l) | ((k == l) & ((x > y) | ((x == y) & (v < w))))))
+
+
 def _plain_select(s):
     case = s["case"]
     n, kin, beams, vocab = case["n"], case["beams_in"], case["beams"], case["vocab"]
     x, scores, stops = s["logits"].view(n, kin, vocab), s["scores"], s["stops"].long()
     largest = x.amax(dim=2, keepdim=True)
     log_sum = largest + torch.log(torch.exp(x - largest).sum(dim=2, keepdim=True))
-    total = (x - log_sum) + scores[:, :, None]
-    total = torch.where(total > -math.inf, total, -math.inf)  # (a row without a likelihood has no candidates)
-    flat = torch.arange(kin * vocab, device=DEVICE)
-    stop_total = total[:, :, stops].reshape(n, kin * len(stops))
-    stop_flat = (torch.arange(kin, device=DEVICE)[:, None] * vocab + stops[None, :]).reshape(-1)
-    total[:, :, stops] = -math.inf
-    width = min(beams, kin * vocab)
-    key, live_at = _key(total.view(n, kin * vocab), flat).topk(width, dim=1)
-    live = total.view(n, -1).gather(1, live_at)
-    if width < beams:
-        live = torch.cat([live, live.new_full((n, beams - width), -math.inf)], 1)
-        key = torch.cat([key, key.new_full((n, beams - width), -(1 << 62))], 1)
-        live_at = torch.cat([live_at, live_at.new_zeros((n, beams - width))], 1)
+    total_of = lambda logit, row: (logit - log_sum[:, :, 0].gather(1, row)) + scores.gather(1, row)  # noqa: E731
+    valid = lambda total: torch.where(total > -math.inf, total, -math.inf)  # noqa: E731  (no likelihood: no candidate)
+    # each row's best tokens that do not end the text, then the best of a sequence's rows
+    on = x.clone()
+    on[:, :, stops] = -math.inf
+    width = min(beams, vocab)
+    token = _key(on, torch.arange(vocab, device=DEVICE)).topk(width, dim=2).indices
+    logit = on.gather(2, token).view(n, kin * width)
+    token = token.view(n, kin * width)
+    parent = torch.arange(kin, device=DEVICE).repeat_interleave(width)[None, :].expand(n, kin * width)
+    live = valid(total_of(logit, parent))
+    best = _key(live, torch.arange(kin * width, device=DEVICE)).topk(min(beams, kin * width), dim=1).indices
+    fill = torch.zeros((n, beams - best.shape[1]), dtype=torch.int64, device=DEVICE)
+    live, parent, token, logit = (torch.cat([t.gather(1, best), (fill - math.inf if t.is_floating_point() else fill).to(t.dtype)], 1)
+                                  for t in (live, parent, token, logit))
     is_live = live > -math.inf
-    parent, token = live_at // vocab, live_at % vocab
+    candidates = (live, parent, logit, token)
     # who continues whom: the best continuation of a beam stays in the beam's place, the others take the free places in order
     order = torch.arange(beams, device=DEVICE)
     earlier = order[None, :, None] > order[None, None, :]
@@ -340,27 +349,32 @@ def _plain_select(s):
     place = torch.where(stays, parent, free_first.gather(1, ((~stays).cumsum(dim=1) - 1).clamp(min=0)))
     idle = torch.clamp(order, max=kin - 1)[None, :].expand(n, beams)  # a place without a beam keeps to itself
     here = torch.empty_like(place).scatter_(1, place, order[None, :].expand(n, beams))
-    live, parent, token, is_live = (t.gather(1, here) for t in (live, parent, token, is_live))
+    next_live, parent, token, is_live = (t.gather(1, here) for t in (live, parent, token, is_live))
     parent, token = torch.where(is_live, parent, idle), torch.where(is_live, token, 0)
     # texts that end here: stop tokens among the first `beams` of all candidates
     length = float(case["produced"] + 1) ** case["penalty"]
     finished, finished_at = s["finished"], s["finished_at"]
     if len(stops) and case["produced"] >= case["min_tokens"]:
-        stop_key, by_key = _key(stop_total, stop_flat).sort(dim=1, descending=True)
-        stop_total, stop_parent = stop_total.gather(1, by_key), (stop_flat // vocab)[by_key]
-        rank = (key[:, None, :] > stop_key[:, :, None]).sum(dim=2) + torch.arange(stop_key.shape[1], device=DEVICE)
-        ended = torch.where((rank < beams) & (stop_total > -math.inf), stop_total / length, -math.inf)
-        at = torch.stack([torch.full_like(stop_parent, case["produced"]), stop_parent], 2).to(torch.int32)
+        stop_parent = torch.arange(kin, device=DEVICE).repeat_interleave(len(stops))[None, :].expand(n, kin * len(stops))
+        stop_logit = x[:, :, stops].reshape(n, kin * len(stops))
+        stop_total = valid(total_of(stop_logit, stop_parent))
+        ending = (stop_total, stop_parent, stop_logit, stops.repeat(kin)[None, :].expand(n, kin * len(stops)))
+        before = _before(ending, ending).sum(dim=2)
+        ended = torch.where((before + _before(candidates, ending).sum(dim=2) < beams) & (stop_total > -math.inf),
+                            stop_total / length, -math.inf)
+        by_rank = before.argsort(dim=1)
+        ended, at = ended.gather(1, by_rank), stop_parent.gather(1, by_rank)
+        at = torch.stack([torch.full_like(at, case["produced"]), at], 2).to(torch.int32)
         at = torch.where((ended > -math.inf)[:, :, None], at, -1)
         pool, by_score = torch.cat([finished, ended], 1).sort(dim=1, descending=True, stable=True)
         finished = pool[:, :beams].contiguous()
         finished_at = torch.cat([finished_at, at], 1).gather(1, by_score[:, :beams, None].expand(n, beams, 2))
-    worst, best = finished[:, -1], live.amax(dim=1)
+    worst, best = finished[:, -1], next_live.amax(dim=1)
     over = (worst > -math.inf) & ((worst >= best / length) | case["early"]) | (best == -math.inf)
     was = s["done"] > 0
     w = was[:, None]
     return {"parents": torch.where(w, idle, parent).to(torch.int32), "tokens": torch.where(w, 0, token).to(torch.int32),
-            "scores": torch.where(w, -math.inf, live), "finished": torch.where(w, s["finished"], finished),
+            "scores": torch.where(w, -math.inf, next_live), "finished": torch.where(w, s["finished"], finished),
             "finished_at": torch.where(w[:, :, None], s["finished_at"], finished_at), "done": (was | over).to(torch.int32)}
 
 
