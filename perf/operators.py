@@ -135,7 +135,7 @@ def _prepare_select(case, g):
     # a few tokens of a row are likely, as after training; so are the stop tokens, now and then
     top = min(24, vocab)
     at = torch.randint(0, vocab, (n * kin, top), generator=g, device=DEVICE)
-    logits.scatter_(1, at, _uniform(g, (n * kin, top), 5.0, 19.0))
+    logits.scatter_reduce_(1, at, _uniform(g, (n * kin, top), 5.0, 19.0), "amax")  # (a place drawn twice: the same in any order)
     stops = torch.arange(case["stops"], device=DEVICE, dtype=torch.int32) * 3 + 2
     logits[:, stops.long()] = _uniform(g, (n * kin, case["stops"]), 0.0, 19.0)
     if case["allowed"] < 1.0:  # what a grammar does not let through
