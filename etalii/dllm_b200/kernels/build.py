@@ -54,6 +54,8 @@ SOURCES = {
     "stream_update": "stream_update.cu",
     "qkv_prepare": "qkv_prepare.cu",
     "sampling": "sampling.cu",
+    "beam_select": "beam_select.cu",
+    "beam_reorder": "beam_reorder.cu",
     "step_launcher": "step_launcher.cu",
 }
 """Library name -> source file. A library added here is built by `build_all` and loadable by `library`."""

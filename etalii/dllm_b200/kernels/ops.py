@@ -255,6 +255,13 @@ _prototypes = {
     ("sampling", "dllm_sample"): [c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p,
                                   c_float, c_int, c_double, c_double, c_void_p],
     ("sampling", "dllm_seed_rng"): [c_void_p, c_void_p, c_void_p, c_int, c_void_p],
+    ("beam_select", "dllm_beam_select_parts"): [c_int, c_int],
+    ("beam_select", "dllm_beam_select"): [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                          c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                          c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float,
+                                          c_int, c_void_p],
+    ("beam_reorder", "dllm_beam_reorder"): [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                                            c_void_p],
 }
 _functions: dict[tuple[str, str], ctypes._CFuncPtr] = {}
 
@@ -2244,6 +2251,91 @@ def seed_rng(rng: torch.Tensor, rows: torch.Tensor, seeds: torch.Tensor) -> None
     assert rng.dtype == torch.int64 and rows.dtype == torch.int32 and seeds.dtype == torch.int64
     _check(_fn("sampling", "dllm_seed_rng")(rng.data_ptr(), rows.data_ptr(), seeds.data_ptr(), rows.numel(),
                                             _stream()), "seed_rng")
+
+
+MAX_BEAMS, MAX_BEAM_STOPS = 32, 8
+"""The most beams of a sequence, and the most stop tokens, that a beam search takes."""
+
+
+def beam_select_scratch(sequences: int, beams_in: int, vocab: int, beams: int) -> int:
+    """Floats of scratch that `beam_select` needs."""
+    rows = sequences * beams_in
+    parts = _fn("beam_select", "dllm_beam_select_parts")(rows, vocab)
+    if parts <= 0:
+        raise KernelError(f"beam_select: {_STATUS.get(parts, parts)}")
+    return rows * parts * (2 + 2 * beams)
+
+
+def beam_select(parents: torch.Tensor, tokens: torch.Tensor, out: tuple, logits: torch.Tensor, state: tuple,
+                produced: torch.Tensor, scratch: torch.Tensor, tickets: torch.Tensor, stop_ids: torch.Tensor | None = None,
+                steps: torch.Tensor | None = None, min_tokens: int = 0, length_penalty: float = 1.0, early: bool = False,
+                history: torch.Tensor | None = None) -> None:
+    """The next beams of every sequence, and the texts that end (the rule: csrc/beam_select.cu).
+
+    logits float32 [sequences * beams_in, vocab]; `state` = (scores float32 [sequences, beams_in], finished float32
+    [sequences, beams] in descending order, -inf where there is none, finished_at int32 [sequences, beams, 2], done int32
+    [sequences]); `out`: the same four for the next step, scores [sequences, beams] (the same tensors where the shapes
+    allow). parents, tokens int32 [sequences, beams]: the beam (of the sequence's) that each place continues, and with which
+    token. A place without a beam has score -inf, itself as parent and token 0. finished_at: (tokens produced before the
+    stop token, the beam that it followed).
+    The beams have produced[0] + steps[0] tokens (int32, `steps` may be None); while those are fewer than `min_tokens` a
+    stop token (`stop_ids` int32, at most MAX_BEAM_STOPS) ends nothing, and it is never a beam's next token. `history`
+    int32 [capacity, sequences, beams]: the parents are kept at history[steps[0]] too. scratch: `beam_select_scratch`
+    floats; tickets: int32 zeros, one a sequence, left zero."""
+    scores, finished, finished_at, done = state
+    scores_out, finished_out, finished_at_out, done_out = out
+    _cuda(parents, tokens, logits, scores, finished, finished_at, done, scores_out, finished_out, finished_at_out, done_out,
+          produced, scratch, tickets, stop_ids, steps, history)
+    sequences, beams_in = scores.shape
+    beams, vocab = parents.shape[1], logits.shape[1]
+    if not 0 < beams <= MAX_BEAMS or not 0 < beams_in <= MAX_BEAMS:
+        raise KernelError(f"beam_select: {beams_in} beams to {beams}: 1 to {MAX_BEAMS}")
+    stops = stop_ids.numel() if stop_ids is not None else 0
+    if stops > MAX_BEAM_STOPS:
+        raise KernelError(f"beam_select: {stops} stop tokens: at most {MAX_BEAM_STOPS}")
+    f32, i32 = torch.float32, torch.int32
+    if not (logits.dtype is f32 and scores.dtype is f32 and finished.dtype is f32 and scores_out.dtype is f32
+            and finished_out.dtype is f32 and scratch.dtype is f32 and parents.dtype is i32 and tokens.dtype is i32
+            and finished_at.dtype is i32 and finished_at_out.dtype is i32 and done.dtype is i32 and done_out.dtype is i32
+            and produced.dtype is i32 and tickets.dtype is i32):
+        raise KernelError("beam_select: logits, scores, finished and scratch are float32, all else int32")
+    if not (logits.shape[0] == sequences * beams_in and parents.shape[0] == sequences and tokens.numel() == parents.numel()
+            and scores_out.numel() == finished.numel() == finished_out.numel() == sequences * beams
+            and finished_at.numel() == finished_at_out.numel() == 2 * sequences * beams
+            and done.numel() == done_out.numel() == sequences and tickets.numel() >= sequences):
+        raise KernelError(f"beam_select: logits {tuple(logits.shape)}, scores {tuple(scores.shape)} and {beams} beams do not "
+                          f"go together with the shapes of the rest")
+    if scratch.numel() < beam_select_scratch(sequences, beams_in, vocab, beams) or scratch.data_ptr() % 8:
+        raise KernelError("beam_select: scratch is too small (beam_select_scratch) or not aligned to 8 bytes")
+    if (stops and stop_ids.dtype is not i32) or (steps is not None and steps.dtype is not i32) or (
+            history is not None and (history.dtype is not i32 or history.numel() % (sequences * beams) or steps is None)):
+        raise KernelError("beam_select: stop_ids, steps and history are int32; history [capacity, sequences, beams] needs steps")
+    _check(_fn("beam_select", "dllm_beam_select")(
+        logits.data_ptr(), logits.stride(0), scores.data_ptr(), finished.data_ptr(), finished_at.data_ptr(), done.data_ptr(),
+        produced.data_ptr(), steps.data_ptr() if steps is not None else None, stop_ids.data_ptr() if stops else None, stops,
+        scores_out.data_ptr(), finished_out.data_ptr(), finished_at_out.data_ptr(), done_out.data_ptr(), parents.data_ptr(),
+        tokens.data_ptr(), history.data_ptr() if history is not None else None,
+        history.numel() // (sequences * beams) if history is not None else 0, scratch.data_ptr(), tickets.data_ptr(),
+        sequences, beams_in, beams, vocab, int(min_tokens), float(length_penalty), int(bool(early)), _stream()),
+        "beam_select", lambda: f"{sequences} sequences of {beams_in} beams: at most 65,535 rows")
+
+
+def beam_reorder(rows, slots: torch.Tensor, parents: torch.Tensor, lengths: torch.Tensor, ahead: int = 0) -> None:
+    """Beam i of sequence b takes over what beam parents[b, i] keeps, all beams at once, in place (csrc/beam_reorder.cu).
+    `rows`: the cache's list (`cache.beams.CacheRows`); slots, parents int32 [sequences, beams]; lengths int32, one a
+    sequence or one a beam (then a sequence's first counts): the positions that its beams have cached, less `ahead`."""
+    _cuda(rows.pieces, slots, parents, lengths)
+    sequences, beams = parents.shape
+    if not 0 < beams <= MAX_BEAMS:
+        raise KernelError(f"beam_reorder: {beams} beams: 1 to {MAX_BEAMS}")
+    if not (slots.dtype is torch.int32 and parents.dtype is torch.int32 and lengths.dtype is torch.int32):
+        raise KernelError("beam_reorder: slots, parents and lengths are int32")
+    each, rest = divmod(lengths.numel(), max(1, sequences))
+    if slots.numel() != sequences * beams or rest or each not in (1, beams):
+        raise KernelError(f"beam_reorder: parents {tuple(parents.shape)}, {slots.numel()} slots, {lengths.numel()} lengths")
+    _check(_fn("beam_reorder", "dllm_beam_reorder")(
+        rows.pieces.data_ptr(), rows.n_pieces, slots.data_ptr(), parents.data_ptr(), lengths.data_ptr(), each, int(ahead),
+        sequences, beams, rows.page_size, _stream()), "beam_reorder", lambda: f"{sequences} sequences: at most 65,535")
 
 
 def decode_advance(tokens: torch.Tensor, tok_pos: torch.Tensor, start: torch.Tensor, chosen: torch.Tensor,
