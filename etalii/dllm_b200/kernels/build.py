@@ -54,6 +54,7 @@ SOURCES = {
     "stream_update": "stream_update.cu",
     "qkv_prepare": "qkv_prepare.cu",
     "sampling": "sampling.cu",
+    "attention_shared": "attention_shared.cu",
     "beam_select": "beam_select.cu",
     "beam_reorder": "beam_reorder.cu",
     "step_launcher": "step_launcher.cu",

@@ -260,6 +260,10 @@ _prototypes = {
                                           c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                           c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float,
                                           c_int, c_void_p],
+    ("attention_shared", "dllm_attention_shared_shape"): [c_int, c_int, c_int, c_int, c_int, c_int, c_int],
+    ("attention_shared", "dllm_attention_shared"): [
+        c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+        c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
     ("beam_reorder", "dllm_beam_reorder"): [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                             c_void_p],
 }
@@ -1669,7 +1673,7 @@ def _status_word() -> torch.Tensor:
 def raise_if_failed() -> None:
     """Raises if a kernel has set the status word since the last look: a bounded wait on an mbarrier ran out
     (codes 2-5 the tile product, 12-21 the tcgen05 attention, 32-33 the product that streams through shared memory, 42-45
-    the experts' tile products), a token saw more keys than its step was prepared for (50),
+    the experts' tile products), a token saw more keys than its step was prepared for (50), a group had more tokens (51),
     or the embedding met a token outside its table (64). Results computed since are not valid. The word lives in
     pinned host memory, so the look costs no synchronisation; it is meaningful after the host has waited for the
     kernels in question (a `.tolist()`, a copy to the host, a synchronize)."""
@@ -1678,6 +1682,8 @@ def raise_if_failed() -> None:
         _async_status[0] = 0
         if code == 64:
             raise KernelError("the embedding was given a token outside its table; the step's results are invalid")
+        if code == 51:
+            raise KernelError("a group has more tokens than its launch was told (max_rows); the step's results are invalid")
         if code == 50:
             raise KernelError("a token sees more keys than the step's max_context; the step's results are invalid")
         raise KernelError(f"a kernel gave up waiting on an mbarrier (role code {code}); the step's results are invalid")
@@ -2382,6 +2388,61 @@ def attention_decode(out: torch.Tensor, q: torch.Tensor, cache, heads: int, scal
         float(scale), int(window or 0), int(chunk), int(batch.max_context), scratch.data_ptr(),
         tickets.data_ptr(), _stream()),
         "attention_decode", lambda: f"head_dim={cache.head_dim} must be a multiple of 8, at most 256")
+
+
+def attention_shared_supported(cache) -> bool:
+    return cache.dtype in _DTYPE_CODE and cache.head_dim % 8 == 0 and cache.head_dim <= 256 and cache.page_size == 64 \
+        and cache.value_dim == cache.head_dim and not cache.keys_only
+
+
+def attention_shared_scratch(cache, heads: int, groups: int, max_rows: int, max_context: int) -> tuple[int, int]:
+    """(floats of scratch, int32 tickets) that `attention_shared` needs for these bounds."""
+    shape = _fn("attention_shared", "dllm_attention_shared_shape")(_code(cache.dtype), heads, cache.kv_heads, cache.head_dim,
+                                                                   groups, max_rows, max_context)
+    if shape <= 0:
+        raise KernelError(f"attention_shared: {_STATUS.get(shape, shape)} ({heads} heads on {cache.kv_heads}, {groups} groups "
+                          f"of {max_rows}, contexts of {max_context})")
+    rows, splits = shape & 0xFFFF, shape >> 16
+    pairs = groups * -(-max_rows * (heads // cache.kv_heads) // rows) * cache.kv_heads
+    return (pairs * splits * rows * (cache.head_dim + 2) if splits > 1 else 0), pairs
+
+
+def attention_shared(out: torch.Tensor, q: torch.Tensor, cache, heads: int, scale: float, window: int, slots: torch.Tensor,
+                     positions: torch.Tensor, groups: torch.Tensor, shared: torch.Tensor, max_rows: int, max_context: int,
+                     scratch: torch.Tensor, tickets: torch.Tensor) -> None:
+    """Attention of a few new tokens a group, where a group's tokens share pages (csrc/attention_shared.cu): the beams of a
+    prompt, or a short chunk appended to a sequence. q, out [tokens, heads * head_dim] in the cache's type (float32 or
+    bfloat16; head sizes that are multiples of 8 up to 256).
+    int32: slots, positions [tokens] (a token's row of the page table, its position; -1 sees nothing and gives zeros);
+    groups [count + 1], the groups' first tokens (they follow one another); shared [count], how many pages from the first on
+    are the same in the table rows of all of a group's tokens (more than there are: all). A group has at most `max_rows` tokens (more:
+    `raise_if_failed` says so) and positions lie below `max_context`. scratch, tickets: `attention_shared_scratch`; the
+    tickets are int32 zeros, left zero."""
+    _cuda(out, q, slots, positions, groups, shared, scratch, tickets)
+    count, tokens, width = groups.numel() - 1, q.shape[0], heads * cache.head_dim
+    if not attention_shared_supported(cache):
+        raise KernelError(f"attention_shared: head_dim {cache.head_dim} (a multiple of 8 up to 256, keys and values alike) in "
+                          f"pages of {cache.page_size} (64) of {cache.dtype}")
+    if q.dtype != cache.dtype or out.dtype != cache.dtype or heads % cache.kv_heads:
+        raise KernelError(f"attention_shared: q {q.dtype}, out {out.dtype}, cache {cache.dtype}; {heads} heads on {cache.kv_heads}")
+    if q.shape[1] != width or out.shape != q.shape or slots.numel() < tokens or positions.numel() < tokens or shared.numel() < count:
+        raise KernelError(f"attention_shared: q {tuple(q.shape)}, out {tuple(out.shape)}, {slots.numel()} slots, "
+                          f"{positions.numel()} positions, {count} groups, {shared.numel()} shared")
+    i32 = torch.int32
+    if not (slots.dtype is i32 and positions.dtype is i32 and groups.dtype is i32 and shared.dtype is i32 and tickets.dtype is i32
+            and scratch.dtype is torch.float32):
+        raise KernelError("attention_shared: scratch is float32, what describes the step int32")
+    floats, words = attention_shared_scratch(cache, heads, max(count, 1), max_rows, max_context)
+    if scratch.numel() < floats or tickets.numel() < words:
+        raise KernelError(f"attention_shared: scratch of {scratch.numel()} floats and {tickets.numel()} tickets: {floats} and {words}")
+    if max_context > cache.max_pages * cache.page_size:
+        raise KernelError(f"attention_shared: contexts of {max_context} in table rows of {cache.max_pages} pages")
+    _check(_fn("attention_shared", "dllm_attention_shared")(
+        out.data_ptr(), q.data_ptr(), cache.base_ptr, cache.page_table.data_ptr(), cache.max_pages, cache.page_size,
+        _code(cache.dtype), heads, cache.kv_heads, cache.head_dim, slots.data_ptr(), positions.data_ptr(), groups.data_ptr(),
+        shared.data_ptr(), count, max_rows, max_context, float(scale), int(window or 0), scratch.data_ptr(), tickets.data_ptr(),
+        _status_word().data_ptr(), _stream()), "attention_shared",
+        lambda: f"{count} groups of {max_rows} tokens, {heads} heads on {cache.kv_heads} of {cache.head_dim}")
 
 
 def attention_prefill_supported(cache) -> bool:
