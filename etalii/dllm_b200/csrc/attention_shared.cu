@@ -19,12 +19,12 @@
 // A masked key has weight 0 by selection, not by arithmetic, and its value is not multiplied: a NaN or infinity in a place
 // that a token does not see leaves it alone. (Products on the tensor cores multiply zeros too: pages that some row
 // sees in part are looked at, and one with a value that is not finite is added element by element.)
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace {
 typedef __nv_bfloat16 bf16;
 constexpr int PAGE = 64;
-constexpr int MAX_ROWS = 64;    // query rows of a tile at most, so tokens too
+constexpr int MAX_ROWS = 128;   // query rows of a tile at most, so tokens too
 constexpr int LIST = 256;       // pages listed at a time
 constexpr int MAX_SPLITS = 128;
 constexpr int FULL = 0x7fffffff;
@@ -73,9 +73,10 @@ __device__ __forceinline__ void make_plan(Plan& p, const Args& a, int rows_per_t
     const int lane = threadIdx.x;
     const int shared = a.shared[group];
     int furthest = -1, which = 0, least_first = FULL, from = 0, to = FULL;
-    int pos[2], low[2], pages[2];
+    constexpr int EACH = MAX_ROWS / 32;
+    int pos[EACH], low[EACH], pages[EACH];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < EACH; ++u) {
       int t = lane + 32 * u;
       pos[u] = -1;
       low[u] = 0;
@@ -107,15 +108,15 @@ __device__ __forceinline__ void make_plan(Plan& p, const Args& a, int rows_per_t
     }
     const int common = min(max(shared, 0), furthest < 0 ? 0 : furthest / PAGE + 1);
     const int shared_count = max(0, common - least_first);
-    int own[2], first_own[2];
+    int own[EACH], first_own[EACH];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < EACH; ++u) {
       first_own[u] = max(common, low[u] / PAGE);
       own[u] = max(0, pages[u] - first_own[u]);
     }
-    int base[2], sum = 0;  // places in the list, tokens in order: lanes hold t and t + 32
+    int base[EACH], sum = 0;  // places in the list, tokens in order: lanes hold t, t + 32, ..
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < EACH; ++u) {
       int through = own[u];
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -144,21 +145,28 @@ __device__ __forceinline__ void make_plan(Plan& p, const Args& a, int rows_per_t
   __syncthreads();
 }
 
+// Place i of the plan's list: whose page it is (-1: the group's) and its index in the table row.
+__device__ __forceinline__ int look_up(const Plan& p, int i, int& whose) {
+  whose = -1;
+  if (i < p.shared_count) return p.shared_first + i;
+  int lo = 0, hi = p.tokens - 1;  // the last token whose own pages begin at or before i
+  while (lo < hi) {
+    int mid = (lo + hi + 1) >> 1;
+    if (p.own_base[mid] <= i) lo = mid;
+    else hi = mid - 1;
+  }
+  whose = lo;
+  return p.own_first[lo] + i - p.own_base[lo];
+}
+__device__ __forceinline__ int page_of(const Plan& p, const Args& a, int whose, int index) {
+  return a.cache.page_table[(size_t)p.slot[whose < 0 ? p.longest : whose] * a.cache.max_pages + index];
+}
+
 // Lists the pages [begin, end) of the plan's list (at most LIST of them). All threads call; ends with a barrier.
 __device__ __forceinline__ void list_pages(Plan& p, const Args& a, int begin, int end) {
   for (int i = begin + (int)threadIdx.x; i < end; i += blockDim.x) {
-    int token = p.longest, index = p.shared_first + i, whose = -1;
-    if (i >= p.shared_count) {
-      int lo = 0, hi = p.tokens - 1;  // the last token whose own pages begin at or before i
-      while (lo < hi) {
-        int mid = (lo + hi + 1) >> 1;
-        if (p.own_base[mid] <= i) lo = mid;
-        else hi = mid - 1;
-      }
-      token = whose = lo;
-      index = p.own_first[lo] + i - p.own_base[lo];
-    }
-    p.page[i - begin] = a.cache.page_table[(size_t)p.slot[token] * a.cache.max_pages + index];
+    int whose, index = look_up(p, i, whose);
+    p.page[i - begin] = page_of(p, a, whose, index);
     p.at[i - begin] = index * PAGE;
     p.whose[i - begin] = whose;
   }
@@ -545,6 +553,376 @@ __global__ void __launch_bounds__(WM * 128) mma_kernel(const Args a) {
   if (is_last(p, a, pair)) join<bf16, ROWS, THREADS>(p, a, pair, reinterpret_cast<float*>(smem_raw));
 }
 
+// ---- 5th-generation tensor cores -----------------------------------------------------------------------------------
+// Scores and outputs in tensor memory, pages by TMA. A product has 128 rows whatever the tile has, so a tile of at most
+// 32 (64) query rows stands in it COPIES = 4 (2) times, one copy above the other, and every copy works on its own 16 (32) of
+// a page's 64 keys: the P tile has the probabilities of those and zeros elsewhere, and the copies' outputs are added at the end.
+// All four warps of a softmax group are then busy with a page, and a thread has 64 / COPIES scores of one query row.
+//   warps 0..7  two softmax groups that take the pages in turn, each with scores, P and outputs of its own: scores from tensor
+//               memory, mask, running maximum (renewed only when a score exceeds it by 2^8) and sum, P as bfloat16 into the
+//               swizzled tile, outputs scaled in tensor memory when the maximum is renewed.
+//   warp 8      looks pages up, 32 at a time, and issues their TMA loads; warp 9 issues the scores' products, warp 10 the outputs'.
+// Pages that some row sees in part are looked at: one with a value that is not finite is added by the softmax warps, key by key,
+// and its product left out.
+// Every wait is bounded; a role that gives up sets the status word and leaves.
+namespace t5 {
+using namespace tc5;
+constexpr int GROUPS = 2, SOFT_WARPS = 4 * GROUPS, THREADS = (SOFT_WARPS + 3) * 32;
+constexpr int P_BYTES = 128 * 128;
+
+template <int BOXES> struct Shape {
+  static constexpr int K_STAGES = BOXES == 2 ? 4 : 3, V_STAGES = BOXES == 2 ? 5 : 4;
+  static constexpr int Q_BYTES = BOXES * 128 * 128, KV_BYTES = BOXES * 64 * 128;
+  static constexpr int OUT = BOXES * 64;                       // columns of the outputs
+  static constexpr unsigned COLUMNS = BOXES == 2 ? 512 : 256;  // of tensor memory
+  static constexpr int SMEM = Q_BYTES + GROUPS * P_BYTES + (K_STAGES + V_STAGES) * KV_BYTES + 1024;
+  static constexpr int LD = OUT + 4;  // floats of a row of the exchange at the end, which lies in P's and the stages' place
+  static_assert(GROUPS * (64 + OUT) <= (int)COLUMNS, "tensor memory");
+  static_assert(GROUPS * 128 * LD * 4 <= GROUPS * P_BYTES + (K_STAGES + V_STAGES) * KV_BYTES, "exchange");
+};
+
+struct Barriers {
+  uint64_t k_full[5], k_empty[5], v_full[5], v_empty[5], s_full[GROUPS], s_empty[GROUPS], p_full[GROUPS], o_full[GROUPS];
+};
+
+template <int BOXES, int COPIES>
+__global__ void __launch_bounds__(THREADS, BOXES == 1 ? 2 : 1) kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
+  typedef Shape<BOXES> S;
+  constexpr int ROWS = 128 / COPIES, KEYS = 64 / COPIES;
+  constexpr int K_STAGES = S::K_STAGES, V_STAGES = S::V_STAGES, KV_BYTES = S::KV_BYTES;
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);  // swizzle atoms: 1 KB
+  unsigned char* q_s = tiles;
+  unsigned char* p_s = q_s + S::Q_BYTES;
+  unsigned char* k_s = p_s + GROUPS * P_BYTES;
+  unsigned char* v_s = k_s + K_STAGES * KV_BYTES;
+  __shared__ Plan p;
+  __shared__ Barriers bar;
+  __shared__ unsigned tmem_base_s;
+  __shared__ float sm_m[GROUPS][128], sm_l[GROUPS][128];
+  __shared__ int odd_s[GROUPS], skip_s[GROUPS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int hd = a.cache.head_dim, kv = blockIdx.y, per_kv = a.heads / a.cache.kv_heads;
+  pdl_launch_dependents();
+  if (tid == 0) {
+    for (int s = 0; s < K_STAGES; ++s) { mbar_init(&bar.k_full[s], 1); mbar_init(&bar.k_empty[s], 1); }
+    for (int s = 0; s < V_STAGES; ++s) { mbar_init(&bar.v_full[s], 1); mbar_init(&bar.v_empty[s], 1); }
+    for (int i = 0; i < GROUPS; ++i) {
+      mbar_init(&bar.s_full[i], 1);
+      mbar_init(&bar.s_empty[i], 4);
+      mbar_init(&bar.p_full[i], 4);
+      mbar_init(&bar.o_full[i], 1);
+      odd_s[i] = skip_s[i] = 0;
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_kv) : "memory");
+  }
+  if (COPIES > 1)  // (what P never gets a value for is zero)
+    for (int i = tid; i < GROUPS * P_BYTES / 16; i += THREADS) reinterpret_cast<uint4*>(p_s)[i] = make_uint4(0u, 0u, 0u, 0u);
+  pdl_wait();
+  make_plan(p, a, ROWS);
+  if (p.rows == 0) return;
+  const size_t pair = (size_t)blockIdx.z * gridDim.y + kv;
+  const int begin = (int)((long long)p.total * blockIdx.x / a.splits), end = (int)((long long)p.total * (blockIdx.x + 1) / a.splits);
+  const int steps = end - begin;
+  if (steps > 0 || a.splits == 1) {
+    if (warp == SOFT_WARPS + 1) tmem_alloc(&tmem_base_s, S::COLUMNS);
+    {  // the queries, once a copy; rows beyond the tile and dimensions beyond the head are zeros
+      const bf16* q = static_cast<const bf16*>(a.q);
+      for (int i = tid; i < ROWS * BOXES * 8; i += THREADS) {
+        int r = i / (BOXES * 8), c = i % (BOXES * 8), row = p.row0 + r;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (r < p.rows && c * 8 < hd)
+          v = *reinterpret_cast<const uint4*>(q + ((size_t)(p.token0 + row / per_kv - p.row0 / per_kv) * a.heads + kv * per_kv + row % per_kv) * hd + c * 8);
+#pragma unroll
+        for (int copy = 0; copy < COPIES; ++copy) {
+          int at = copy * ROWS + r;
+          *reinterpret_cast<uint4*>(q_s + (c >> 3) * 16384 + at * 128 + (((c & 7) ^ (at & 7)) << 4)) = v;
+        }
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const unsigned tmem_s = tmem_base_s, tmem_o = tmem_base_s + GROUPS * 64;
+    if (warp == SOFT_WARPS) {
+      int issued_k = 0, issued_v = 0;
+      bool ok = true;
+      for (int j0 = 0; j0 < steps && ok; j0 += 32) {
+        int page = 0;
+        if (j0 + lane < steps) {
+          int whose, index = look_up(p, begin + j0 + lane, whose);
+          page = page_of(p, a, whose, index);
+        }
+        for (int u = 0; u < 32 && j0 + u < steps && ok; ++u) {
+          const int j = j0 + u, sk = j % K_STAGES, sv = j % V_STAGES;
+          const int at = __shfl_sync(0xffffffffu, page, u);
+          if (lane == 0) {
+            const int row_k = ((at * 2 + 0) * a.cache.kv_heads + kv) * PAGE, row_v = ((at * 2 + 1) * a.cache.kv_heads + kv) * PAGE;
+            if (j >= K_STAGES && !mbar_wait(&bar.k_empty[sk], (j / K_STAGES - 1) & 1)) ok = false;
+            if (ok) {
+              mbar_expect_tx(&bar.k_full[sk], KV_BYTES);
+#pragma unroll
+              for (int x = 0; x < BOXES; ++x) tma_load_2d(k_s + sk * KV_BYTES + x * 8192, &map_kv, &bar.k_full[sk], x * 64, row_k);
+              issued_k = j + 1;
+              if (j >= V_STAGES && !mbar_wait(&bar.v_empty[sv], (j / V_STAGES - 1) & 1)) ok = false;
+            }
+            if (ok) {
+              mbar_expect_tx(&bar.v_full[sv], KV_BYTES);
+#pragma unroll
+              for (int x = 0; x < BOXES; ++x) tma_load_2d(v_s + sv * KV_BYTES + x * 8192, &map_kv, &bar.v_full[sv], x * 64, row_v);
+              issued_v = j + 1;
+            }
+          }
+          ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        }
+      }
+      if (!ok && lane == 0) {  // gave up: nothing may land in this block's shared memory after it has left
+        *(volatile int*)a.status = 52;
+        for (int j = max(0, issued_k - K_STAGES); j < issued_k; ++j) mbar_wait(&bar.k_full[j % K_STAGES], (j / K_STAGES) & 1);
+        for (int j = max(0, issued_v - V_STAGES); j < issued_v; ++j) mbar_wait(&bar.v_full[j % V_STAGES], (j / V_STAGES) & 1);
+      }
+    } else if (warp == SOFT_WARPS + 1) {
+      if (lane == 0) {
+        constexpr unsigned idesc = instr_desc(128, 64);
+        const unsigned q_addr = smem_u32(q_s);
+        for (int i = 0; i < steps; ++i) {
+          const int g = i % GROUPS, s = i % K_STAGES;
+          if (!mbar_wait(&bar.k_full[s], (i / K_STAGES) & 1) || (i >= GROUPS && !mbar_wait(&bar.s_empty[g], (i / GROUPS - 1) & 1))) {
+            *(volatile int*)a.status = 53;
+            break;
+          }
+          fence_after_sync();
+          const unsigned k_addr = smem_u32(k_s + s * KV_BYTES);
+#pragma unroll
+          for (int k = 0; k < BOXES * 4; ++k)
+            if (k * 16 < hd)
+              umma(tmem_s + (unsigned)(g * 64), smem_desc(q_addr + (k >> 2) * 16384 + (k & 3) * 32),
+                   smem_desc(k_addr + (k >> 2) * 8192 + (k & 3) * 32), idesc, k > 0 ? 1u : 0u);
+          tcgen05_commit(&bar.k_empty[s]);
+          tcgen05_commit(&bar.s_full[g]);
+        }
+      }
+    } else if (warp == SOFT_WARPS + 2) {
+      if (lane == 0) {
+        constexpr unsigned idesc = instr_desc(128, 64, true);
+        for (int i = 0; i < steps; ++i) {
+          const int g = i % GROUPS, s = i % V_STAGES;
+          if (!mbar_wait(&bar.p_full[g], (i / GROUPS) & 1) || !mbar_wait(&bar.v_full[s], (i / V_STAGES) & 1)) {
+            *(volatile int*)a.status = 54;
+            break;
+          }
+          fence_after_sync();
+          if (!*(volatile int*)&skip_s[g]) {
+            const unsigned p_addr = smem_u32(p_s + g * P_BYTES), v_addr = smem_u32(v_s + s * KV_BYTES);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+              for (int x = 0; x < BOXES; ++x)
+                umma(tmem_o + (unsigned)(g * S::OUT + x * 64), smem_desc(p_addr + k * 32), smem_desc(v_addr + x * 8192 + k * 2048), idesc,
+                     (k > 0 || i >= GROUPS) ? 1u : 0u);
+          }
+          tcgen05_commit(&bar.v_empty[s]);
+          tcgen05_commit(&bar.o_full[g]);
+        }
+      }
+    } else {
+      const int g = warp >> 2, r = (warp & 3) * 32 + lane, row = r % ROWS, first_key = r / ROWS * KEYS;
+      const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
+      const unsigned s_addr = tmem_s + lanes + (unsigned)(g * 64 + first_key), o_addr = tmem_o + lanes + (unsigned)(g * S::OUT);
+      unsigned char* p_row = p_s + g * P_BYTES + r * 128;
+      const bool real = row < p.rows;
+      const int token = real ? (p.row0 + row) / per_kv - p.row0 / per_kv : -2;
+      const int high = real ? p.position[token] : -1, low = real ? p.low[token] : 0;
+      const float scale = a.scale * 1.4426950408889634f;
+      float m_run = -INFINITY, l_run = 0.f;
+      bool ok = true;
+      int taken = 0;
+      // (a wait that ran out is not left at once: the warps of a group meet at barriers that they all have to reach)
+      for (int j = g; j < steps; j += GROUPS, ++taken) {
+        int whose;
+        const int at = look_up(p, begin + j, whose) * PAGE;
+        const bool edge = whose >= 0 || at < p.all_from || at + PAGE - 1 > p.all_to;
+        ok = ok && mbar_wait(&bar.s_full[g], (j / GROUPS) & 1);
+        __syncwarp();
+        fence_after_sync();
+        float v[KEYS];
+#pragma unroll
+        for (int c = 0; c < KEYS; c += 16) tmem_load16_nowait(s_addr + (unsigned)c, reinterpret_cast<unsigned*>(v) + c);
+        tmem_wait_ld();
+        fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.s_empty[g]);
+#pragma unroll
+        for (int c = 0; c < KEYS; ++c) v[c] *= scale;
+        unsigned long long seen = ~0ull;
+        if (edge) {
+          const bool mine = whose < 0 || whose == token;
+          seen = 0ull;
+#pragma unroll
+          for (int c = 0; c < KEYS; ++c) {
+            const int key = at + first_key + c;
+            const bool sees = mine && key <= high && key >= low;
+            if (sees) seen |= 1ull << c;
+            else v[c] = -INFINITY;
+          }
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < KEYS; ++c) mx[c & 3] = fmaxf(mx[c & 3], v[c]);
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        float fade = 1.f;
+        if (top > m_run + 8.f) {  // (also a row's first scores, while its maximum is still -inf)
+          fade = fast_exp2(m_run - top);
+          m_run = top;
+        }
+        const float shift = m_run > -INFINITY ? m_run : 0.f;
+        unsigned packed[KEYS / 2];
+#pragma unroll
+        for (int c = 0; c < KEYS; c += 2) {
+          const float w0 = fast_exp2(v[c] - shift), w1 = fast_exp2(v[c + 1] - shift);
+          sum[c & 3] += w0;
+          sum[(c + 1) & 3] += w1;
+          packed[c / 2] = pack_bf16(w0, w1);
+        }
+        l_run = l_run * fade + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+        // the group's previous product has to be over: it reads P and adds to the outputs
+        if (taken >= 1) {
+          ok = ok && mbar_wait(&bar.o_full[g], ((j - GROUPS) / GROUPS) & 1);
+          __syncwarp();
+          fence_after_sync();
+        }
+#pragma unroll
+        for (int c = 0; c < KEYS / 8; ++c)
+          *reinterpret_cast<uint4*>(p_row + (((first_key / 8 + c) ^ (r & 7)) << 4)) =
+              make_uint4(packed[4 * c], packed[4 * c + 1], packed[4 * c + 2], packed[4 * c + 3]);
+        bool odd = false;
+        const unsigned char* v_tile = v_s + (j % V_STAGES) * KV_BYTES;
+        if (edge) {
+          ok = ok && mbar_wait(&bar.v_full[j % V_STAGES], (j / V_STAGES) & 1);
+#pragma unroll
+          for (int i = 0; i < KV_BYTES / 16 / 128; ++i) {
+            uint4 x = *reinterpret_cast<const uint4*>(v_tile + (i * 128 + r) * 16);
+            odd = odd || odd_pair(x.x) || odd_pair(x.y) || odd_pair(x.z) || odd_pair(x.w);
+          }
+          if (__any_sync(0xffffffffu, odd) && lane == 0) odd_s[g] = 1;
+          asm volatile("bar.sync %0, 128;" ::"r"(2 + g) : "memory");
+          odd = *(volatile int*)&odd_s[g] != 0;
+          asm volatile("bar.sync %0, 128;" ::"r"(2 + g) : "memory");
+          if (r == 0) { odd_s[g] = 0; *(volatile int*)&skip_s[g] = odd; }
+        } else if (r == 0) {
+          *(volatile int*)&skip_s[g] = 0;
+        }
+        if (odd || (taken >= 1 && __any_sync(0xffffffffu, fade != 1.f))) {
+#pragma unroll 1
+          for (int c = 0; c < S::OUT; c += 16) {
+            unsigned o[16];
+            if (taken >= 1) tmem_load16(o_addr + (unsigned)c, o);
+#pragma unroll
+            for (int d = 0; d < 16; ++d) o[d] = taken >= 1 ? __float_as_uint(__uint_as_float(o[d]) * fade) : 0u;
+            if (odd) {
+#pragma unroll 1
+              for (int key = 0; key < KEYS; ++key) {
+                if (!(seen >> key & 1ull)) continue;
+                const int at_key = first_key + key;
+                const float w = __bfloat162float(*reinterpret_cast<const bf16*>(p_row + (((at_key >> 3) ^ (r & 7)) << 4) + 2 * (at_key & 7)));
+#pragma unroll
+                for (int d = 0; d < 16; ++d) {
+                  const int column = (c & 63) + d;
+                  const bf16 x = *reinterpret_cast<const bf16*>(v_tile + (c >> 6) * 8192 + at_key * 128 + (((column >> 3) ^ (at_key & 7)) << 4) + 2 * (column & 7));
+                  o[d] = __float_as_uint(fmaf(w, __bfloat162float(x), __uint_as_float(o[d])));
+                }
+              }
+              __syncwarp();
+            }
+            tmem_store16(o_addr + (unsigned)c, o);
+          }
+          tmem_wait_st();
+          fence_before_sync();
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.p_full[g]);
+      }
+      if (ok && taken >= 1) ok = mbar_wait(&bar.o_full[g], (taken - 1) & 1);
+      if (!ok) *(volatile int*)a.status = 55;
+      __syncwarp();
+      fence_after_sync();
+      // ---- groups and copies together: a common maximum, then sums through shared memory (P and the stages are free: every
+      // product has been added)
+      sm_m[g][r] = m_run;
+      sm_l[g][r] = l_run;
+      asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < GROUPS; ++i)
+#pragma unroll
+        for (int copy = 0; copy < COPIES; ++copy) top = fmaxf(top, sm_m[i][copy * ROWS + row]);
+      const float w = m_run > -INFINITY ? fast_exp2(m_run - top) : 0.f;
+      float* ex = reinterpret_cast<float*>(p_s);
+#pragma unroll 1
+      for (int c = 0; c < S::OUT; c += 16) {
+        unsigned o[16];
+        if (taken >= 1) tmem_load16(o_addr + (unsigned)c, o);
+#pragma unroll
+        for (int d = 0; d < 16; d += 4) {
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (taken >= 1 && w != 0.f)
+            x = make_float4(__uint_as_float(o[d]) * w, __uint_as_float(o[d + 1]) * w, __uint_as_float(o[d + 2]) * w, __uint_as_float(o[d + 3]) * w);
+          *reinterpret_cast<float4*>(ex + (size_t)(g * 128 + r) * S::LD + c + d) = x;
+        }
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
+      const int fours = hd / 4;
+      for (int i = tid; i < p.rows * fours; i += SOFT_WARPS * 32) {
+        const int to = i / fours, d = (i % fours) * 4;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        float most = -INFINITY, total = 0.f;
+#pragma unroll
+        for (int e = 0; e < GROUPS * COPIES; ++e) most = fmaxf(most, sm_m[e / COPIES][e % COPIES * ROWS + to]);
+#pragma unroll
+        for (int e = 0; e < GROUPS * COPIES; ++e) {
+          const int from = e % COPIES * ROWS + to;
+          float4 y = *reinterpret_cast<const float4*>(ex + (size_t)(e / COPIES * 128 + from) * S::LD + d);
+          x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+          const float me = sm_m[e / COPIES][from], le = sm_l[e / COPIES][from];
+          total += me > -INFINITY ? le * fast_exp2(me - most) : le;
+        }
+        if (a.splits == 1) {
+          const float inv = total != 0.f ? 1.f / total : 0.f;
+          const int in_group = p.row0 + to, t = p.token0 + in_group / per_kv - p.row0 / per_kv;
+          *reinterpret_cast<uint2*>(static_cast<bf16*>(a.out) + ((size_t)t * a.heads + kv * per_kv + in_group % per_kv) * hd + d) =
+              make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
+        } else {
+          *reinterpret_cast<float4*>(a.scratch + ((pair * a.splits + blockIdx.x) * ROWS + to) * hd + d) = x;
+          if (d == 0) {
+            float* ml = a.scratch + (size_t)gridDim.z * gridDim.y * a.splits * ROWS * hd + ((pair * a.splits + blockIdx.x) * ROWS + to) * 2;
+            *reinterpret_cast<float2*>(ml) = make_float2(most, total);
+          }
+        }
+      }
+    }
+    fence_before_sync();
+    __syncthreads();
+    if (warp == SOFT_WARPS + 1) tmem_dealloc(tmem_base_s, S::COLUMNS);
+  }
+  if (a.splits == 1) return;
+  if (is_last(p, a, pair)) join<bf16, ROWS, THREADS>(p, a, pair, reinterpret_cast<float*>(tiles));
+}
+
+template <int BOXES, int COPIES>
+int launch(const Args& a, long long pages, dim3 grid, cudaStream_t stream) {
+  typedef Shape<BOXES> S;
+  static_assert((MAX_SPLITS + 1) * 128 * 4 + 1024 <= S::SMEM, "the weights of the join");
+  CUtensorMap map;
+  if (!make_map(&map, a.cache.base, pages * 2 * a.cache.kv_heads * PAGE, a.cache.head_dim, PAGE)) return DLLM_LAUNCH_FAILED;
+  static std::atomic<unsigned long long> done{0};
+  if (!dllm_allow_shared((const void*)kernel<BOXES, COPIES>, S::SMEM, done)) return DLLM_LAUNCH_FAILED;
+  return dllm_launch_pdl(kernel<BOXES, COPIES>, grid, dim3(THREADS), S::SMEM, stream, map, a);
+}
+}  // namespace t5
+
 // ---- everything else ---------------------------------------------------------------------------------------------
 // 16 query rows a tile, 128 threads. A page's keys, then its values, lie in shared memory as float32. Scores: a thread has one
 // key and half of the rows; the softmax: a warp four rows; the sums: a thread four dimensions and some of the rows.
@@ -707,20 +1085,26 @@ __global__ void __launch_bounds__(FMA_THREADS) fma_kernel(const Args a) {
 }
 
 // ---- launch shapes -------------------------------------------------------------------------------------------------
-struct Shape { int rows, tiles, splits; bool mma; };
+enum { FMA = 0, MMA = 1, TCGEN05 = 2 };
+struct Shape { int kind, rows, tiles, splits; };
 
-Shape shape_of(int dtype, int heads, int kv_heads, int head_dim, int groups, int max_rows, int max_context) {
+// `kind`: -1 chooses.
+Shape shape_of(int kind, int dtype, int heads, int kv_heads, int head_dim, int groups, int max_rows, int max_context) {
   Shape s;
   const int query_rows = max_rows * (heads / kv_heads);
-  s.mma = dtype == DLLM_BF16 && head_dim % 16 == 0 && head_dim <= 128;
-  s.rows = !s.mma ? FMA_ROWS : query_rows <= 16 ? 16 : query_rows <= 32 ? 32 : 64;
+  const bool mma = dtype == DLLM_BF16 && head_dim % 16 == 0 && head_dim <= 128, tcgen05 = mma && head_dim >= 64;
+  const int pages = (max_context + PAGE - 1) / PAGE;
+  s.kind = kind >= 0 ? kind : tcgen05 && pages > 4 ? TCGEN05 : mma ? MMA : FMA;
+  if ((s.kind == TCGEN05 && !tcgen05) || (s.kind == MMA && !mma)) s.kind = FMA;
+  if (s.kind == FMA) s.rows = FMA_ROWS;
+  else if (s.kind == MMA) s.rows = query_rows <= 16 ? 16 : query_rows <= 32 ? 32 : 64;
+  else s.rows = query_rows <= 32 ? 32 : query_rows <= 64 ? 64 : 128;
   s.tiles = (query_rows + s.rows - 1) / s.rows;
   // as many splits as the device has places for, but not more than there can be pages
   const long long pairs = (long long)groups * s.tiles * kv_heads;
-  const long long places = 148LL * 2;
+  const long long places = 148LL * (s.kind == TCGEN05 && head_dim > 64 ? 1 : 2);
   long long splits = places / (pairs > 0 ? pairs : 1);
-  const long long pages = (max_context + PAGE - 1) / PAGE + max_rows;
-  if (splits > pages) splits = pages;
+  if (splits > pages + max_rows) splits = pages + max_rows;
   if (splits > MAX_SPLITS) splits = MAX_SPLITS;
   s.splits = splits < 1 ? 1 : (int)splits;
   return s;
@@ -748,28 +1132,44 @@ int launch_fma(const Args& a, dim3 grid, cudaStream_t stream) {
 }  // namespace
 
 // Query rows of a tile in the low 16 bits, splits above: scratch holds groups x tiles x kv_heads x splits x rows x
-// (head_dim + 2) floats, tickets groups x tiles x kv_heads words.
-DLLM_EXPORT int dllm_attention_shared_shape(int dtype, int heads, int kv_heads, int head_dim, int groups, int max_rows, int max_context) {
+// (head_dim + 2) floats, tickets groups x tiles x kv_heads words. kind: -1, or 0, 1, 2 (fused multiply-adds, mma.sync, tcgen05).
+DLLM_EXPORT int dllm_attention_shared_shape(int kind, int dtype, int heads, int kv_heads, int head_dim, int groups, int max_rows,
+                                            int max_context) {
   if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || groups <= 0 || max_rows <= 0 || max_context <= 0) return DLLM_BAD_ARGUMENT;
-  Shape s = shape_of(dtype, heads, kv_heads, head_dim, groups, max_rows, max_context);
+  Shape s = shape_of(kind, dtype, heads, kv_heads, head_dim, groups, max_rows, max_context);
   return s.rows | s.splits << 16;
 }
 
 // See the head of the file. out, q [tokens, heads * head_dim] in the cache's type; slots, positions: each token's table row and
-// position; cuts [groups + 1]: the groups' first tokens; shared [groups]: pages from the first on that a group's table rows have in common.
-DLLM_EXPORT int dllm_attention_shared(void* out, const void* q, void* base, const int* page_table, int max_pages, int page_size,
-                                      int dtype, int heads, int kv_heads, int head_dim, const int* slots, const int* positions,
-                                      const int* cuts, const int* shared, int groups, int max_rows, int max_context, float scale,
-                                      int window, float* scratch, unsigned* tickets, int* status, cudaStream_t stream) {
+// position; cuts [groups + 1]: the groups' first tokens; shared [groups]: pages from the first on that a group's table rows have
+// in common; the cache entry has `pages` pages.
+DLLM_EXPORT int dllm_attention_shared(int kind, void* out, const void* q, void* base, long long pages, const int* page_table,
+                                      int max_pages, int page_size, int dtype, int heads, int kv_heads, int head_dim,
+                                      const int* slots, const int* positions, const int* cuts, const int* shared, int groups,
+                                      int max_rows, int max_context, float scale, int window, float* scratch, unsigned* tickets,
+                                      int* status, cudaStream_t stream) {
   if (groups <= 0 || max_rows <= 0) return DLLM_OK;
-  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_context <= 0 || window < 0) return DLLM_BAD_ARGUMENT;
-  if (head_dim % 8 || head_dim <= 0 || head_dim > FMA_DIM || page_size != PAGE || kv_heads > 65535) return DLLM_UNSUPPORTED_SIZE;
-  Shape s = shape_of(dtype, heads, kv_heads, head_dim, groups, max_rows, max_context);
+  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_context <= 0 || window < 0 || pages <= 0) return DLLM_BAD_ARGUMENT;
+  if (head_dim % 8 || head_dim <= 0 || head_dim > FMA_DIM || page_size != PAGE || kv_heads > 65535 ||
+      ((uintptr_t)out | (uintptr_t)q | (uintptr_t)base) & 15)
+    return DLLM_UNSUPPORTED_SIZE;
+  Shape s = shape_of(kind, dtype, heads, kv_heads, head_dim, groups, max_rows, max_context);
   if ((long long)groups * s.tiles > 65535) return DLLM_UNSUPPORTED_SIZE;
   Args a{out, q, KvLayout{base, page_table, max_pages, page_size, kv_heads, head_dim}, slots, positions, cuts, shared, scratch,
          tickets, status, heads, window, s.tiles, s.splits, scale};
   dim3 grid(s.splits, kv_heads, groups * s.tiles);
-  if (!s.mma) return dtype == DLLM_BF16 ? launch_fma<bf16>(a, grid, stream) : launch_fma<float>(a, grid, stream);
+  if (s.kind == FMA) return dtype == DLLM_BF16 ? launch_fma<bf16>(a, grid, stream) : launch_fma<float>(a, grid, stream);
+  if (s.kind == TCGEN05) {
+    if (pages * 2 * kv_heads * PAGE > 0x7fffffffll) return DLLM_UNSUPPORTED_SIZE;
+    if (head_dim <= 64) {
+      if (s.rows == 32) return t5::launch<1, 4>(a, pages, grid, stream);
+      if (s.rows == 64) return t5::launch<1, 2>(a, pages, grid, stream);
+      return t5::launch<1, 1>(a, pages, grid, stream);
+    }
+    if (s.rows == 32) return t5::launch<2, 4>(a, pages, grid, stream);
+    if (s.rows == 64) return t5::launch<2, 2>(a, pages, grid, stream);
+    return t5::launch<2, 1>(a, pages, grid, stream);
+  }
   if (head_dim <= 32) {
     if (s.rows == 16) return launch_mma<32, 1, 1, 4>(a, grid, stream);
     if (s.rows == 32) return launch_mma<32, 2, 1, 4>(a, grid, stream);
