@@ -1,20 +1,21 @@
 // Attention of a few new tokens a group over the paged cache, where the tokens of a group share pages: the beams of one
 // prompt (the prompt's pages in common, pages of their own behind them), or the tokens of a short chunk that is appended to
-// one sequence (all pages in common, each token sees up to itself). Pages in common are read once for all tokens of the
-// group and all query heads of the key/value head; the others once for each token.
+// one sequence (all pages in common, each token sees up to itself). A page is read once for all tokens of the group that have
+// it and all query heads of the key/value head.
 //
 //   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q.k_j - max),  over the positions j <= position of the token's own
 //   table row (and j > position - window). A token at position -1 sees nothing: zeros.
 //
-// A group's query rows (tokens x query heads of one kv head, in that order) are cut into tiles of ROWS. What a tile has to read is
-// a list of pages: those in common, then each token's own. The list is cut into `splits` stretches of equal length, a block
-// each, so that the device is filled whatever the contexts are; running maximum and sum are kept in float32. Partial results go to
-// scratch, and the block that finishes last for its tile and kv head (a ticket; nobody waits) joins them in order.
+// A group's query rows (tokens x query heads of one kv head, in that order) are cut into tiles. What a tile has to read is
+// a list of pages: those in common, then the tokens' own, each once for the tokens that have it. The list is cut into
+// `splits` stretches of equal length, a block each, so that the device is filled whatever the contexts are; running maximum
+// and sum are kept in float32. Up to eight blocks form a cluster and add their results up through distributed shared memory; where there
+// are more clusters, theirs go to scratch and the block that finishes last for its tile and kv head (a ticket; nobody
+// waits) joins them in order.
 //
-// bfloat16, head sizes that are multiples of 16 up to 128: tensor cores (mma.sync). Pages travel by cp.async through a
-// ring of stages; the four warps that share a tile's rows take 16 of a page's 64 keys each, with a maximum and a sum of
-// their own, so that no page costs a barrier between softmax and product. Probabilities are rounded to bfloat16 as the second
-// product's operand. Everything else (float32, other head sizes): fused multiply-adds on pages in shared memory.
+// bfloat16, head sizes that are multiples of 16: from 64 to 128 on the 5th-generation tensor cores (namespace t5), below
+// with mma.sync (mma_kernel). Probabilities are rounded to bfloat16 as the second product's operand. Everything else
+// (float32, other head sizes): fused multiply-adds on pages in shared memory (fma_kernel).
 //
 // A masked key has weight 0 by selection, not by arithmetic, and its value is not multiplied: a NaN or infinity in a place
 // that a token does not see leaves it alone. (Products on the tensor cores multiply zeros too: pages that some row
@@ -26,7 +27,7 @@ typedef __nv_bfloat16 bf16;
 constexpr int PAGE = 64;
 constexpr int MAX_ROWS = 128;   // query rows of a tile at most, so tokens too
 constexpr int LIST = 256;       // pages listed at a time
-constexpr int MAX_SPLITS = 128;
+constexpr int MAX_CLUSTER = 8, MAX_CLUSTERS = 32;
 constexpr int FULL = 0x7fffffff;
 constexpr int TOO_MANY = 51;    // status: a group has more tokens than the launch was told
 
@@ -35,10 +36,10 @@ struct Args {
   const void* q;
   KvLayout cache;
   const int *slots, *positions, *cuts, *shared;
-  float* scratch;      // [tile, kv head][split][ROWS][head_dim], then [..][ROWS][2]
+  float* scratch;      // [tile, kv head][cluster][ROWS][head_dim], then [..][ROWS][2]
   unsigned* tickets;   // one a (tile, kv head), zero between launches
   int* status;
-  int heads, window, tiles, splits;
+  int heads, window, tiles, splits, cluster;  // blocks of a tile and kv head; of a cluster
   float scale;
 };
 
@@ -48,10 +49,13 @@ struct Plan {
   int row0, rows;                // its query rows, counted from the group's first
   int shared_first, shared_count, total;
   int longest;                   // the token that sees furthest: its table row names the pages in common
-  int all_from, all_to;          // positions that every token sees
+  int all_from, all_to;          // positions that every token sees (of those that see any)
   int position[MAX_ROWS], low[MAX_ROWS], slot[MAX_ROWS];   // of each token: it sees low .. position
-  int own_first[MAX_ROWS], own_base[MAX_ROWS + 1];         // its pages behind those in common: first, place in the list
-  int page[LIST], at[LIST], whose[LIST];                   // a stretch of the list: page, first position, token or -1
+  // The pages behind those in common, each once: page, index in the table row, which tokens have it (a bit each, all bits:
+  // everybody). Only where the tile has at most 32 tokens and they fit; else (listed -1) a token's pages follow one
+  // another: list_index has each token's first own page, list_page its place in the list.
+  int listed, list_page[LIST], list_index[LIST];
+  unsigned list_who[LIST];
   int last;
 };
 
@@ -59,168 +63,251 @@ struct Plan {
 __device__ __forceinline__ void make_plan(Plan& p, const Args& a, int rows_per_tile) {
   const int group = blockIdx.z / a.tiles, tile = blockIdx.z % a.tiles;
   const int per_kv = a.heads / a.cache.kv_heads;
-  const int first = a.cuts[group], count = a.cuts[group + 1] - first;
-  const int row0 = tile * rows_per_tile, rows = min(rows_per_tile, count * per_kv - row0);
-  if (threadIdx.x == 0 && tile == a.tiles - 1 && count * per_kv > a.tiles * rows_per_tile)
-    *reinterpret_cast<volatile int*>(a.status) = TOO_MANY;  // (the launch was made for fewer tokens a group)
-  if (rows <= 0) {
-    if (threadIdx.x == 0) { p.rows = 0; p.total = 0; }
-    __syncthreads();
-    return;
-  }
-  const int t0 = row0 / per_kv, tokens = (row0 + rows - 1) / per_kv - t0 + 1;
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
-    const int shared = a.shared[group];
-    int furthest = -1, which = 0, least_first = FULL, from = 0, to = FULL;
-    constexpr int EACH = MAX_ROWS / 32;
-    int pos[EACH], low[EACH], pages[EACH];
+    const int first = a.cuts[group], count = a.cuts[group + 1] - first, shared = a.shared[group];
+    const int row0 = tile * rows_per_tile, rows = min(rows_per_tile, count * per_kv - row0);
+    if (lane == 0) {
+      if (tile == a.tiles - 1 && count * per_kv > a.tiles * rows_per_tile)
+        *reinterpret_cast<volatile int*>(a.status) = TOO_MANY;  // (the launch was made for fewer tokens a group)
+      p.rows = max(rows, 0);
+      p.total = 0;
+    }
+    if (rows > 0) {
+      const int t0 = row0 / per_kv, tokens = (row0 + rows - 1) / per_kv - t0 + 1;
+      constexpr int EACH = MAX_ROWS / 32;
+      int furthest = -1, which = 0, least_first = FULL, from = 0, to = FULL;
+      int pos[EACH], low[EACH], pages[EACH], slot[EACH];
 #pragma unroll
-    for (int u = 0; u < EACH; ++u) {
-      int t = lane + 32 * u;
-      pos[u] = -1;
-      low[u] = 0;
-      int slot = 0;
-      if (t < tokens) {
-        pos[u] = a.positions[first + t0 + t];
-        slot = a.slots[first + t0 + t];
-        if (slot < 0) { slot = 0; pos[u] = -1; }
+      for (int u = 0; u < EACH; ++u) {
+        const int t = lane + 32 * u;
+        pos[u] = t < tokens ? a.positions[first + t0 + t] : -1;
+        slot[u] = t < tokens ? a.slots[first + t0 + t] : -1;
+      }
+#pragma unroll
+      for (int u = 0; u < EACH; ++u) {
+        const int t = lane + 32 * u;
+        if (slot[u] < 0) { slot[u] = 0; pos[u] = -1; }
         pos[u] = min(pos[u], a.cache.max_pages * PAGE - 1);
         low[u] = a.window > 0 ? max(0, pos[u] + 1 - a.window) : 0;
-        from = max(from, low[u]);
-        to = min(to, pos[u]);
-        p.position[t] = pos[u];
-        p.low[t] = low[u];
-        p.slot[t] = slot;
+        pages[u] = pos[u] < 0 ? 0 : pos[u] / PAGE + 1;
+        if (t < tokens) {
+          p.position[t] = pos[u];
+          p.low[t] = low[u];
+          p.slot[t] = slot[u];
+        }
+        if (pos[u] >= 0) {  // (what a token that sees nothing gets is set aside at the end)
+          from = max(from, low[u]);
+          to = min(to, pos[u]);
+          least_first = min(least_first, low[u] / PAGE);
+          if (pos[u] > furthest) { furthest = pos[u]; which = t; }
+        }
       }
-      pages[u] = pos[u] / PAGE + 1;
-      if (pos[u] < 0) pages[u] = 0;
-      if (pos[u] > furthest) { furthest = pos[u]; which = t; }
-      if (pages[u]) least_first = min(least_first, low[u] / PAGE);
-    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      int f = __shfl_xor_sync(0xffffffffu, furthest, o), w = __shfl_xor_sync(0xffffffffu, which, o);
-      if (f > furthest || (f == furthest && w < which)) { furthest = f; which = w; }
-      least_first = min(least_first, __shfl_xor_sync(0xffffffffu, least_first, o));
-      from = max(from, __shfl_xor_sync(0xffffffffu, from, o));
-      to = min(to, __shfl_xor_sync(0xffffffffu, to, o));
-    }
-    const int common = min(max(shared, 0), furthest < 0 ? 0 : furthest / PAGE + 1);
-    const int shared_count = max(0, common - least_first);
-    int own[EACH], first_own[EACH];
-#pragma unroll
-    for (int u = 0; u < EACH; ++u) {
-      first_own[u] = max(common, low[u] / PAGE);
-      own[u] = max(0, pages[u] - first_own[u]);
-    }
-    int base[EACH], sum = 0;  // places in the list, tokens in order: lanes hold t, t + 32, ..
-#pragma unroll
-    for (int u = 0; u < EACH; ++u) {
-      int through = own[u];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        int other = __shfl_up_sync(0xffffffffu, through, o);
-        if (lane >= o) through += other;
+      for (int o = 16; o > 0; o >>= 1) {
+        int f = __shfl_xor_sync(0xffffffffu, furthest, o), w = __shfl_xor_sync(0xffffffffu, which, o);
+        if (f > furthest || (f == furthest && w < which)) { furthest = f; which = w; }
+        least_first = min(least_first, __shfl_xor_sync(0xffffffffu, least_first, o));
+        from = max(from, __shfl_xor_sync(0xffffffffu, from, o));
+        to = min(to, __shfl_xor_sync(0xffffffffu, to, o));
       }
-      base[u] = sum + through - own[u];
-      sum += __shfl_sync(0xffffffffu, through, 31);
-      int t = lane + 32 * u;
-      if (t < tokens) { p.own_first[t] = first_own[u]; p.own_base[t] = shared_count + base[u]; }
-    }
-    if (lane == 0) {
-      p.token0 = first + t0;
-      p.tokens = tokens;
-      p.row0 = row0;
-      p.rows = rows;
-      p.shared_first = least_first;
-      p.shared_count = shared_count;
-      p.total = shared_count + sum;
-      p.own_base[tokens] = shared_count + sum;
-      p.longest = which;
-      p.all_from = from;
-      p.all_to = to;
+      const int all = furthest < 0 ? 0 : furthest / PAGE + 1, common = min(max(shared, 0), all);
+      const int shared_count = max(0, common - least_first);
+      int total = shared_count, listed = -1;
+      if (tokens <= 32) {
+        // a lane a token, eight indexes of the table rows at a time: tokens with the same page share an entry
+        const unsigned everybody = __ballot_sync(0xffffffffu, pages[0] > 0);
+        listed = 0;
+        for (int i0 = max(common, least_first); i0 < all && listed >= 0; i0 += 8) {
+          int page[8];
+#pragma unroll
+          for (int n = 0; n < 8; ++n) {
+            const int i = i0 + n;
+            const bool has = i < pages[0] && i >= low[0] / PAGE;
+            page[n] = has ? a.cache.page_table[(size_t)slot[0] * a.cache.max_pages + i] : -1 - lane;
+          }
+#pragma unroll
+          for (int n = 0; n < 8; ++n) {
+            const int i = i0 + n;
+            const bool has = i < pages[0] && i >= low[0] / PAGE;
+            const unsigned same = __match_any_sync(0xffffffffu, page[n]);
+            const bool leads = has && (same & ((1u << lane) - 1u)) == 0u;
+            const unsigned leaders = __ballot_sync(0xffffffffu, leads);
+            const int at = listed + __popc(leaders & ((1u << lane) - 1u));
+            if (leads && at < LIST) {
+              p.list_page[at] = page[n];
+              p.list_index[at] = i;
+              p.list_who[at] = same == everybody ? 0xffffffffu : same;
+            }
+            listed += __popc(leaders);
+          }
+          if (listed > LIST) listed = -1;
+        }
+        if (listed >= 0) total += listed;
+      }
+      if (listed < 0) {
+        int base = shared_count;  // places in the list, tokens in order: lanes hold t, t + 32, ..
+#pragma unroll
+        for (int u = 0; u < EACH; ++u) {
+          const int t = lane + 32 * u, first_own = max(common, low[u] / PAGE), own = max(0, pages[u] - first_own);
+          int through = own;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            int other = __shfl_up_sync(0xffffffffu, through, o);
+            if (lane >= o) through += other;
+          }
+          if (t < tokens) { p.list_index[t] = first_own; p.list_page[t] = base + through - own; }
+          base += __shfl_sync(0xffffffffu, through, 31);
+        }
+        total = base;
+      }
+      if (lane == 0) {
+        p.token0 = first + t0;
+        p.tokens = tokens;
+        p.row0 = row0;
+        p.shared_first = least_first;
+        p.shared_count = shared_count;
+        p.total = total;
+        p.listed = listed;
+        p.longest = which;
+        p.all_from = from;
+        p.all_to = to;
+      }
     }
   }
   __syncthreads();
 }
 
-// Place i of the plan's list: whose page it is (-1: the group's) and its index in the table row.
-__device__ __forceinline__ int look_up(const Plan& p, int i, int& whose) {
-  whose = -1;
+// Who has a page: everybody (EVERYBODY), else a bit a token where the plan lists pages, else one token.
+constexpr int EVERYBODY = -1;
+__device__ __forceinline__ bool has_page(const Plan& p, int who, int token) {
+  return who == EVERYBODY || (p.listed >= 0 ? ((unsigned)who >> (token & 31) & 1u) != 0u : who == token);
+}
+// Place i of the list: who has the page, and its index in the table rows.
+__device__ __forceinline__ int look_up(const Plan& p, int i, int& who) {
+  who = EVERYBODY;
   if (i < p.shared_count) return p.shared_first + i;
+  if (p.listed >= 0) {
+    who = (int)p.list_who[i - p.shared_count];
+    return p.list_index[i - p.shared_count];
+  }
   int lo = 0, hi = p.tokens - 1;  // the last token whose own pages begin at or before i
   while (lo < hi) {
     int mid = (lo + hi + 1) >> 1;
-    if (p.own_base[mid] <= i) lo = mid;
+    if (p.list_page[mid] <= i) lo = mid;
     else hi = mid - 1;
   }
-  whose = lo;
-  return p.own_first[lo] + i - p.own_base[lo];
+  who = lo;
+  return p.list_index[lo] + i - p.list_page[lo];
 }
-__device__ __forceinline__ int page_of(const Plan& p, const Args& a, int whose, int index) {
-  return a.cache.page_table[(size_t)p.slot[whose < 0 ? p.longest : whose] * a.cache.max_pages + index];
+__device__ __forceinline__ int page_at(const Plan& p, const Args& a, int i) {
+  if (i >= p.shared_count && p.listed >= 0) return p.list_page[i - p.shared_count];
+  int who, index = look_up(p, i, who);
+  return a.cache.page_table[(size_t)p.slot[who == EVERYBODY ? p.longest : who] * a.cache.max_pages + index];
 }
 
-// Lists the pages [begin, end) of the plan's list (at most LIST of them). All threads call; ends with a barrier.
-__device__ __forceinline__ void list_pages(Plan& p, const Args& a, int begin, int end) {
+// A stretch of the list, at most LIST pages: page, first position, who has it.
+struct Stretch { int page[LIST], at[LIST], who[LIST]; };
+// (All threads call; ends with a barrier.)
+__device__ __forceinline__ void fill(Stretch& l, const Plan& p, const Args& a, int begin, int end) {
   for (int i = begin + (int)threadIdx.x; i < end; i += blockDim.x) {
-    int whose, index = look_up(p, i, whose);
-    p.page[i - begin] = page_of(p, a, whose, index);
-    p.at[i - begin] = index * PAGE;
-    p.whose[i - begin] = whose;
+    l.at[i - begin] = look_up(p, i, l.who[i - begin]) * PAGE;
+    l.page[i - begin] = page_at(p, a, i);
   }
   __syncthreads();
 }
 
-// The last block of a tile and kv head joins the partial results of all splits, in order. weight: ROWS x splits floats of shared memory.
-template <typename T, int ROWS, int THREADS>
-__device__ __forceinline__ void join(const Plan& p, const Args& a, size_t pair, float* weight) {
-  const int hd = a.cache.head_dim, splits = a.splits, per_kv = a.heads / a.cache.kv_heads;
-  const float* part = a.scratch + pair * splits * ROWS * hd;
-  const float* ml = a.scratch + (size_t)gridDim.z * gridDim.y * splits * ROWS * hd + pair * splits * ROWS * 2;
-  auto empty = [&](int s) { return (long long)p.total * s / splits == (long long)p.total * (s + 1) / splits; };
-  for (int r = threadIdx.x; r < p.rows; r += THREADS) {
-    float top = -INFINITY, sum = 0.f;
-    for (int s = 0; s < splits; ++s)
-      if (!empty(s)) top = fmaxf(top, __ldcg(ml + (s * ROWS + r) * 2));
-    for (int s = 0; s < splits; ++s) {
-      float w = 0.f;
-      if (!empty(s)) {
-        float2 pair_ml = __ldcg(reinterpret_cast<const float2*>(ml + (s * ROWS + r) * 2));
-        w = pair_ml.x > -INFINITY ? exp2f(pair_ml.x - top) : 0.f;
-        if (pair_ml.x > -INFINITY || pair_ml.y != 0.f) sum += pair_ml.x > -INFINITY ? w * pair_ml.y : pair_ml.y;
-      }
-      weight[s * ROWS + r] = w;
-    }
-    weight[splits * ROWS + r] = sum != 0.f ? 1.f / sum : 0.f;
-  }
-  __syncthreads();
-  const int pieces = hd / 4;
-  for (int i = threadIdx.x; i < p.rows * pieces; i += THREADS) {
-    int r = i / pieces, d = (i % pieces) * 4;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < splits; ++s) {
-      float w = weight[s * ROWS + r];
-      if (w == 0.f) continue;
-      float4 v = __ldcg(reinterpret_cast<const float4*>(part + ((size_t)s * ROWS + r) * hd + d));
-      acc.x = fmaf(w, v.x, acc.x);
-      acc.y = fmaf(w, v.y, acc.y);
-      acc.z = fmaf(w, v.z, acc.z);
-      acc.w = fmaf(w, v.w, acc.w);
-    }
-    float inv = weight[splits * ROWS + r];
-    int row = p.row0 + r, token = p.token0 + row / per_kv - p.row0 / per_kv, head = blockIdx.y * per_kv + row % per_kv;
-    T* to = static_cast<T*>(a.out) + ((size_t)token * a.heads + head) * hd + d;
-    to[0] = from_float<T>(acc.x * inv);
-    to[1] = from_float<T>(acc.y * inv);
-    to[2] = from_float<T>(acc.z * inv);
-    to[3] = from_float<T>(acc.w * inv);
+// ---- results: of a block, of a cluster, of all ------------------------------------------------------------------------
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n"
+               "barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ unsigned remote_addr(const void* local, unsigned rank) {
+  unsigned addr = (unsigned)__cvta_generic_to_shared(local), remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+  return remote;
+}
+__device__ __forceinline__ float2 remote_float2(unsigned addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 remote_float4(unsigned addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// (maximum, sum) of partial results together, the maxima as powers of two: what a part counts, and the sum. A sum beside a
+// maximum of -inf is 0, or a NaN that has to stay one.
+__device__ __forceinline__ float share_of(float m, float top) { return m > -INFINITY ? exp2f(m - top) : 0.f; }
+
+template <typename T>
+__device__ __forceinline__ void write_out(const Plan& p, const Args& a, int r, int d, float4 x, float sum) {
+  const int per_kv = a.heads / a.cache.kv_heads, row = p.row0 + r, token = p.token0 + row / per_kv - p.row0 / per_kv;
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
+  T* to = static_cast<T*>(a.out) + ((size_t)token * a.heads + blockIdx.y * per_kv + row % per_kv) * a.cache.head_dim + d;
+  if (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(to) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+  } else {
+    __nv_bfloat162 pair[2] = {__floats2bfloat162_rn(x.x * inv, x.y * inv), __floats2bfloat162_rn(x.z * inv, x.w * inv)};
+    *reinterpret_cast<uint2*>(to) = *reinterpret_cast<uint2*>(pair);
   }
 }
 
-// Is this block the last of its tile and kv head? (All threads call.)
-__device__ __forceinline__ bool is_last(Plan& p, const Args& a, size_t pair) {
+// Every block has its result in shared memory: x[row * ld ..] sums, ml[row] (maximum, sum); a block without pages has (-inf, 0)
+// there and anything in x. The blocks of the cluster take the rows' pieces in turn. All threads call.
+template <typename T, int ROWS>
+__device__ __forceinline__ void finish(Plan& p, const Args& a, const float* x, int ld, const float2* ml, float* weight) {
+  const int hd = a.cache.head_dim, fours = hd / 4, clusters = a.splits / a.cluster;
+  const unsigned size = a.cluster, rank = blockIdx.x % size;
+  const size_t pair = (size_t)blockIdx.z * gridDim.y + blockIdx.y;
+  float* parts = a.scratch;
+  float* part_ml = a.scratch + (size_t)gridDim.z * gridDim.y * clusters * ROWS * hd;
+  if (size > 1) cluster_sync();
+  else __syncthreads();
+  for (int i = rank * blockDim.x + threadIdx.x; i < p.rows * fours; i += size * blockDim.x) {
+    const int r = i / fours, d = (i % fours) * 4;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    float top = -INFINITY, total = 0.f;
+    if (size == 1) {
+      sum = *reinterpret_cast<const float4*>(x + r * ld + d);
+      top = ml[r].x;
+      total = ml[r].y;
+      if (top == -INFINITY) sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    } else {
+      float2 each[MAX_CLUSTER];
+      float4 v[MAX_CLUSTER];
+#pragma unroll
+      for (unsigned c = 0; c < MAX_CLUSTER; ++c)
+        if (c < size) {
+          each[c] = remote_float2(remote_addr(ml + r, c));
+          v[c] = remote_float4(remote_addr(x + r * ld + d, c));
+        }
+#pragma unroll
+      for (unsigned c = 0; c < MAX_CLUSTER; ++c)
+        if (c < size) top = fmaxf(top, each[c].x);
+#pragma unroll
+      for (unsigned c = 0; c < MAX_CLUSTER; ++c)
+        if (c < size) {
+          const float w = share_of(each[c].x, top);
+          total += each[c].x > -INFINITY ? w * each[c].y : each[c].y;
+          if (w != 0.f) {
+            sum.x = fmaf(w, v[c].x, sum.x); sum.y = fmaf(w, v[c].y, sum.y);
+            sum.z = fmaf(w, v[c].z, sum.z); sum.w = fmaf(w, v[c].w, sum.w);
+          }
+        }
+    }
+    if (clusters == 1) {
+      write_out<T>(p, a, r, d, sum, total);
+    } else {
+      const size_t at = (pair * clusters + blockIdx.x / size) * ROWS + r;
+      *reinterpret_cast<float4*>(parts + at * hd + d) = sum;
+      if (d == 0) *reinterpret_cast<float2*>(part_ml + at * 2) = make_float2(top, total);
+    }
+  }
+  if (size > 1) cluster_sync();  // nobody leaves while others read its result
+  if (clusters == 1) return;
   __threadfence();
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -228,8 +315,37 @@ __device__ __forceinline__ bool is_last(Plan& p, const Args& a, size_t pair) {
     if (p.last) a.tickets[pair] = 0u;
   }
   __syncthreads();
+  if (!p.last) return;
   __threadfence();
-  return p.last != 0;
+  // the last block: what each cluster's part counts [cluster][row], then the rows' sums
+  float2* all_ml = reinterpret_cast<float2*>(weight);
+  for (int i = threadIdx.x; i < clusters * ROWS; i += blockDim.x)
+    if (i % ROWS < p.rows) all_ml[i] = __ldcg(reinterpret_cast<const float2*>(part_ml) + pair * clusters * ROWS + i);
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.rows * fours; i += blockDim.x) {
+    const int r = i / fours, d = (i % fours) * 4;
+    float top = -INFINITY, total = 0.f;
+    for (int c = 0; c < clusters; ++c) top = fmaxf(top, all_ml[c * ROWS + r].x);
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c0 = 0; c0 < clusters; c0 += 4) {
+      float4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (c0 + u < clusters) v[u] = __ldcg(reinterpret_cast<const float4*>(parts + ((pair * clusters + c0 + u) * ROWS + r) * hd + d));
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (c0 + u < clusters) {
+          const float2 each = all_ml[(c0 + u) * ROWS + r];
+          const float w = share_of(each.x, top);
+          total += each.x > -INFINITY ? w * each.y : each.y;
+          if (w != 0.f) {
+            sum.x = fmaf(w, v[u].x, sum.x); sum.y = fmaf(w, v[u].y, sum.y);
+            sum.z = fmaf(w, v[u].z, sum.z); sum.w = fmaf(w, v[u].w, sum.w);
+          }
+        }
+    }
+    write_out<T>(p, a, r, d, sum, total);
+  }
 }
 
 // ---- tensor cores ------------------------------------------------------------------------------------------------
@@ -260,23 +376,25 @@ __device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<unsigned*>(&v);
 }
-// one of two packed bfloat16 is not finite
-__device__ __forceinline__ bool odd_pair(unsigned v) {
-  return (v & 0x7f80u) == 0x7f80u || (v & 0x7f800000u) == 0x7f800000u;
-}
+// Packed bfloat16: the sign bit's place of each that is not finite (an exponent of all ones carries into it); other bits mean
+// nothing.
+__device__ __forceinline__ unsigned odd_bits(unsigned v) { return (v & 0x7f807f80u) + 0x00800080u; }
+__device__ __forceinline__ bool any_odd(unsigned bits) { return (bits & 0x80008000u) != 0u; }
 // where piece `c` (16 bytes) of row r lies: neighbouring rows' pieces in different banks
 template <int HD> __device__ __forceinline__ int place(int r, int c) {
   return r * HD + 8 * (HD >= 64 ? c ^ (r & 7) : c ^ ((r >> 1) & 3));
 }
 
-// HD: the head size, padded (32, 64, 128). A warp has 16 * MT query rows; WM warps (of 4) lie one above another in the tile.
+// HD: the head size, padded (32, 64). A warp has 16 * MT query rows; WM warps (of 4) lie one above another in the tile.
 template <int HD, int MT, int WM, int STAGES>
 __global__ void __launch_bounds__(WM * 128) mma_kernel(const Args a) {
   constexpr int THREADS = WM * 128, ROWS = 16 * MT * WM;
   constexpr bool KEEP_Q = MT * HD <= 128;  // the queries' operands stay in registers
   extern __shared__ __align__(128) unsigned char smem_raw[];
   __shared__ Plan p;
+  __shared__ Stretch list;
   __shared__ float sm_m[4][ROWS], sm_l[4][ROWS];
+  __shared__ float2 sm_ml[ROWS];
   bf16* q_s = reinterpret_cast<bf16*>(smem_raw);  // [ROWS][HD]
   bf16* ring = q_s + ROWS * HD;                    // per stage: keys [64][HD], values [64][HD]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -286,9 +404,9 @@ __global__ void __launch_bounds__(WM * 128) mma_kernel(const Args a) {
   pdl_wait();
   make_plan(p, a, ROWS);
   if (p.rows == 0) return;
-  const size_t pair = (size_t)blockIdx.z * gridDim.y + kv;
   const int begin = (int)((long long)p.total * blockIdx.x / a.splits), end = (int)((long long)p.total * (blockIdx.x + 1) / a.splits);
-  if (begin < end || a.splits == 1) {
+  float* sum = reinterpret_cast<float*>(ring);  // [4][ROWS][HD], at the end
+  if (begin < end) {
     // queries (rows beyond the tile and dimensions beyond the head are zeros)
     const bf16* q = static_cast<const bf16*>(a.q);
     for (int i = tid; i < ROWS * (HD / 8); i += THREADS) {
@@ -314,7 +432,7 @@ __global__ void __launch_bounds__(WM * 128) mma_kernel(const Args a) {
         bool real = r < p.rows;
         int t = real ? (p.row0 + r) / per_kv - p.row0 / per_kv : 0;
         token[i][e] = real ? t : -2;
-        high[i][e] = real ? p.position[t] : FULL;
+        high[i][e] = real ? p.position[t] : -1;
         low[i][e] = real ? p.low[t] : 0;
       }
     float m[MT][2], l[MT][2], o[MT][HD / 8][4];
@@ -333,17 +451,15 @@ __global__ void __launch_bounds__(WM * 128) mma_kernel(const Args a) {
 
     for (int part = begin; part < end; part += LIST) {
       const int count = min(LIST, end - part);
-      list_pages(p, a, part, part + count);
+      fill(list, p, a, part, part + count);
       auto bring = [&](int i) {
         bf16* keys = ring + (size_t)(i % STAGES) * 2 * 64 * HD;
-        int page = p.page[i], at = p.at[i], whose = p.whose[i];
-        // what nobody sees is not read: zeros lie there
-        int from = whose < 0 ? at : p.low[whose], to = whose < 0 ? p.position[p.longest] : p.position[whose];
-        const bf16* src = base + kv_offset(a.cache, page, 0, kv, 0);
+        const int left = p.position[p.longest] - list.at[i];  // (rows that nobody sees are not read)
+        const bf16* src = base + kv_offset(a.cache, list.page[i], 0, kv, 0);
         const size_t values = (size_t)a.cache.kv_heads * PAGE * hd;
         for (int c = tid; c < 64 * (HD / 8); c += THREADS) {
           int r = c / (HD / 8), d = c % (HD / 8);
-          bool ok = at + r >= from && at + r <= to;
+          const bool ok = r <= left;
           if (d < pieces) {
             cp_async_16(keys + place<HD>(r, d), ok ? src + r * hd + d * 8 : base, ok);
             cp_async_16(keys + 64 * HD + place<HD>(r, d), ok ? src + values + r * hd + d * 8 : base, ok);
@@ -369,8 +485,8 @@ __global__ void __launch_bounds__(WM * 128) mma_kernel(const Args a) {
             for (int k = 0; k < (KEEP_Q ? HD / 16 : 1); ++k)
               ldmatrix_x4(qf[i][k], q_s + place<HD>(16 * (MT * tier + i) + (lane & 15), 2 * k + (lane >> 4)));
         }
-        const int whose = p.whose[it], at = p.at[it] + 16 * quarter;
-        const bool whole = whose < 0 && at >= p.all_from && at + 15 <= p.all_to;
+        const int who = list.who[it], at = list.at[it] + 16 * quarter;
+        const bool whole = who == EVERYBODY && at >= p.all_from && at + 15 <= p.all_to;
         float s[MT][2][4];
 #pragma unroll
         for (int i = 0; i < MT; ++i)
@@ -400,6 +516,7 @@ __global__ void __launch_bounds__(WM * 128) mma_kernel(const Args a) {
           for (int e = 0; e < 2; ++e) {
             float top = m[i][e];
             seen[i][e] = 15u;
+            const bool mine = whole || (token[i][e] >= 0 && has_page(p, who, token[i][e]));
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -407,7 +524,7 @@ __global__ void __launch_bounds__(WM * 128) mma_kernel(const Args a) {
                 float v = s[i][j][2 * e + u] * scale;
                 if (!whole) {
                   int key = at + 8 * j + 2 * (lane & 3) + u;
-                  bool sees = key <= high[i][e] && key >= low[i][e] && (whose < 0 || whose == token[i][e]);
+                  bool sees = mine && key <= high[i][e] && key >= low[i][e];
                   if (!sees) {
                     v = -INFINITY;
                     seen[i][e] &= ~(1u << (2 * j + u));
@@ -448,13 +565,14 @@ __global__ void __launch_bounds__(WM * 128) mma_kernel(const Args a) {
         }
         bool odd = false;
         if (!whole) {  // does a value that somebody may not see have to be kept out of the product?
+          unsigned bits = 0u;
 #pragma unroll
           for (int n = 0; n < HD / 16; ++n) {
             unsigned vf[4];
             ldmatrix_x4_trans(vf, vals + place<HD>(16 * quarter + (lane & 15), 2 * n + (lane >> 4)));
-            odd = odd || odd_pair(vf[0]) || odd_pair(vf[1]) || odd_pair(vf[2]) || odd_pair(vf[3]);
+            bits |= odd_bits(vf[0]) | odd_bits(vf[1]) | odd_bits(vf[2]) | odd_bits(vf[3]);
           }
-          odd = __any_sync(0xffffffffu, odd);
+          odd = __any_sync(0xffffffffu, any_odd(bits));
         }
         if (!odd) {
 #pragma unroll
@@ -498,20 +616,20 @@ __global__ void __launch_bounds__(WM * 128) mma_kernel(const Args a) {
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
+        if (high[i][e] < 0) { m[i][e] = -INFINITY; l[i][e] = 0.f; }  // (a row that sees nothing)
         l[i][e] += __shfl_xor_sync(0xffffffffu, l[i][e], 1);
         l[i][e] += __shfl_xor_sync(0xffffffffu, l[i][e], 2);
         int r = 16 * (MT * tier + i) + (lane >> 2) + 8 * e;
         if ((lane & 3) == 0) { sm_m[quarter][r] = m[i][e]; sm_l[quarter][r] = l[i][e]; }
       }
     __syncthreads();
-    float* sum = reinterpret_cast<float*>(ring);  // [4][ROWS][HD]
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         int r = 16 * (MT * tier + i) + (lane >> 2) + 8 * e;
         float top = fmaxf(fmaxf(sm_m[0][r], sm_m[1][r]), fmaxf(sm_m[2][r], sm_m[3][r]));
-        float w = m[i][e] > -INFINITY ? exp2f(m[i][e] - top) : 0.f;
+        float w = share_of(m[i][e], top);
         // (rows without a key in this quarter: nothing, whatever the products made of zeros)
 #pragma unroll
         for (int n = 0; n < HD / 8; ++n) {
@@ -521,75 +639,134 @@ __global__ void __launch_bounds__(WM * 128) mma_kernel(const Args a) {
         }
       }
     __syncthreads();
-    const int fours = hd / 4;
-    for (int i = tid; i < p.rows * fours; i += THREADS) {
-      int r = i / fours, d = (i % fours) * 4;
+    for (int i = tid; i < ROWS * (HD / 4); i += THREADS) {  // (into the first quarter's place)
+      const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      float top = -INFINITY, total = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) top = fmaxf(top, sm_m[w][r]);
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         float4 x = *reinterpret_cast<const float4*>(sum + ((size_t)w * ROWS + r) * HD + d);
         v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
-        total += sm_m[w][r] > -INFINITY ? sm_l[w][r] * exp2f(sm_m[w][r] - top) : sm_l[w][r];
       }
-      if (a.splits == 1) {
-        float inv = total != 0.f ? 1.f / total : 0.f;
-        int row = p.row0 + r, t = p.token0 + row / per_kv - p.row0 / per_kv;
-        uint2 packed = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
-        *reinterpret_cast<uint2*>(static_cast<bf16*>(a.out) + ((size_t)t * a.heads + kv * per_kv + row % per_kv) * hd + d) = packed;
-      } else {
-        float* part = a.scratch + ((pair * a.splits + blockIdx.x) * ROWS + r) * hd + d;
-        *reinterpret_cast<float4*>(part) = v;
-        if (d == 0) {
-          float* ml = a.scratch + (size_t)gridDim.z * gridDim.y * a.splits * ROWS * hd + ((pair * a.splits + blockIdx.x) * ROWS + r) * 2;
-          *reinterpret_cast<float2*>(ml) = make_float2(top, total);
-        }
+      *reinterpret_cast<float4*>(sum + (size_t)r * HD + d) = v;
+      if (d == 0) {
+        float top = -INFINITY, total = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, sm_m[w][r]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) total += sm_m[w][r] > -INFINITY ? sm_l[w][r] * exp2f(sm_m[w][r] - top) : sm_l[w][r];
+        sm_ml[r] = make_float2(top, total);
       }
     }
+  } else {
+    for (int r = tid; r < ROWS; r += THREADS) sm_ml[r] = make_float2(-INFINITY, 0.f);
   }
-  if (a.splits == 1) return;
-  if (is_last(p, a, pair)) join<bf16, ROWS, THREADS>(p, a, pair, reinterpret_cast<float*>(smem_raw));
+  finish<bf16, ROWS>(p, a, sum, HD, sm_ml, reinterpret_cast<float*>(q_s));
+}
+
+template <typename Kernel, typename... Rest>
+int launch_clusters(Kernel kernel, dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream, const Rest&... rest) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attributes[2];
+  int n = 0;
+  if (cluster > 1) {
+    attributes[n].id = cudaLaunchAttributeClusterDimension;
+    attributes[n].val.clusterDim.x = cluster;
+    attributes[n].val.clusterDim.y = 1;
+    attributes[n++].val.clusterDim.z = 1;
+  }
+  if (dllm_pdl_enabled()) {
+    attributes[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  config.attrs = attributes;
+  config.numAttrs = n;
+  return cudaLaunchKernelEx(&config, kernel, rest...) == cudaSuccess ? DLLM_OK : DLLM_LAUNCH_FAILED;
 }
 
 // ---- 5th-generation tensor cores -----------------------------------------------------------------------------------
-// Scores and outputs in tensor memory, pages by TMA. A product has 128 rows whatever the tile has, so a tile of at most
-// 32 (64) query rows stands in it COPIES = 4 (2) times, one copy above the other, and every copy works on its own 16 (32) of
-// a page's 64 keys: the P tile has the probabilities of those and zeros elsewhere, and the copies' outputs are added at the end.
-// All four warps of a softmax group are then busy with a page, and a thread has 64 / COPIES scores of one query row.
-//   warps 0..7  two softmax groups that take the pages in turn, each with scores, P and outputs of its own: scores from tensor
-//               memory, mask, running maximum (renewed only when a score exceeds it by 2^8) and sum, P as bfloat16 into the
-//               swizzled tile, outputs scaled in tensor memory when the maximum is renewed.
-//   warp 8      looks pages up, 32 at a time, and issues their TMA loads; warp 9 issues the scores' products, warp 10 the outputs'.
-// Pages that some row sees in part are looked at: one with a value that is not finite is added by the softmax warps, key by key,
-// and its product left out.
+// A step takes two pages, 128 keys. The query rows are few, so keys and values are the operands of 128 rows and the query
+// rows the columns of both products: S^T = K Q^T (keys x rows), O^T += V^T P^T (dimensions x rows; keys and values as they lie in
+// their pages, P^T written as [key][row]). A product then reads 128 x 16 values of a page and ROWS x 16 others; with the query
+// rows as the 128-row operand (padded) it would read those 128 x 16 for every 64 keys: 768 cycles of shared memory a page
+// for heads of 128 instead of 320.
+//   softmax warps  two groups that take the steps in turn, each with scores, P and outputs of its own: a thread has a key
+//                  and 32 query rows. A row's maximum over the step goes through redux and shared memory; where it grew the
+//                  group's outputs are scaled in tensor memory (32 columns). Every step uses the running maximum itself, so
+//                  that the largest weight is 1 and not rounded.
+//   three more     one looks pages up, 32 at a time, and issues their TMA loads; one issues the scores' products, one the
+//                  outputs'.
+// Pages that some row sees in part are looked at: a value that is not finite is kept out of the product; such a step is added
+// by the softmax warps, key by key.
 // Every wait is bounded; a role that gives up sets the status word and leaves.
 namespace t5 {
 using namespace tc5;
-constexpr int GROUPS = 2, SOFT_WARPS = 4 * GROUPS, THREADS = (SOFT_WARPS + 3) * 32;
-constexpr int P_BYTES = 128 * 128;
+constexpr int KEYS = 2 * PAGE;
+constexpr int P_BYTES = KEYS * 128;  // [key][64 rows]
 
-template <int BOXES> struct Shape {
-  static constexpr int K_STAGES = BOXES == 2 ? 4 : 3, V_STAGES = BOXES == 2 ? 5 : 4;
-  static constexpr int Q_BYTES = BOXES * 128 * 128, KV_BYTES = BOXES * 64 * 128;
-  static constexpr int OUT = BOXES * 64;                       // columns of the outputs
-  static constexpr unsigned COLUMNS = BOXES == 2 ? 512 : 256;  // of tensor memory
+template <int BOXES, int ROWS> struct Shape {
+  static constexpr int GROUPS = BOXES == 1 && ROWS == 32 ? 3 : 2;
+  static constexpr int HALVES = ROWS / 32;                      // warps that share a step's keys, 32 rows each
+  static constexpr int GROUP = 4 * HALVES, SOFT_WARPS = GROUPS * GROUP, THREADS = (SOFT_WARPS + 3) * 32;
+  static constexpr int K_STAGES = BOXES == 2 ? 2 : 4, V_STAGES = BOXES == 2 ? 3 : 5;
+  static constexpr int Q_BYTES = BOXES * ROWS * 128, KV_BYTES = BOXES * KEYS * 128;
+  static constexpr unsigned COLUMNS = 2 * GROUPS * ROWS > 128 ? 256 : 128;  // of tensor memory: scores and outputs
   static constexpr int SMEM = Q_BYTES + GROUPS * P_BYTES + (K_STAGES + V_STAGES) * KV_BYTES + 1024;
-  static constexpr int LD = OUT + 4;  // floats of a row of the exchange at the end, which lies in P's and the stages' place
-  static_assert(GROUPS * (64 + OUT) <= (int)COLUMNS, "tensor memory");
-  static_assert(GROUPS * 128 * LD * 4 <= GROUPS * P_BYTES + (K_STAGES + V_STAGES) * KV_BYTES, "exchange");
+  static constexpr int LD = BOXES * 64 + 4;  // floats of a row of the results at the end, which lie in the stages' place
+  static_assert(GROUPS * ROWS * LD * 4 <= (K_STAGES + V_STAGES) * KV_BYTES, "results");
 };
 
 struct Barriers {
-  uint64_t k_full[5], k_empty[5], v_full[5], v_empty[5], s_full[GROUPS], s_empty[GROUPS], p_full[GROUPS], o_full[GROUPS];
+  uint64_t k_full[4], k_empty[4], v_full[5], v_empty[5], s_full[4], s_empty[4], p_full[4], o_full[4];
 };
 
-template <int BOXES, int COPIES>
-__global__ void __launch_bounds__(THREADS, BOXES == 1 ? 2 : 1) kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
-  typedef Shape<BOXES> S;
-  constexpr int ROWS = 128 / COPIES, KEYS = 64 / COPIES;
-  constexpr int K_STAGES = S::K_STAGES, V_STAGES = S::V_STAGES, KV_BYTES = S::KV_BYTES;
+// An operand whose rows of 128 bytes (64 values of M or N) are its K index; `next`: bytes from 64 values of M or N to the next.
+__device__ __forceinline__ uint64_t transposed_desc(unsigned addr, unsigned next) {
+  return (smem_desc(addr) & ~((uint64_t)0x3FFF << 16)) | ((uint64_t)(next >> 4) << 16);
+}
+__device__ __forceinline__ float largest_of_warp(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// two floats at a time
+typedef unsigned long long Two;
+__device__ __forceinline__ Two two(float x, float y) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 apart(Two v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+template <int BOXES, int ROWS>
+__global__ void __launch_bounds__(Shape<BOXES, ROWS>::THREADS, 1)
+    kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
+  typedef Shape<BOXES, ROWS> S;
+  constexpr int GROUPS = S::GROUPS, K_STAGES = S::K_STAGES, V_STAGES = S::V_STAGES, KV_BYTES = S::KV_BYTES, SOFT_WARPS = S::SOFT_WARPS;
+  constexpr int BOX = KEYS * 128;  // bytes of 64 columns of a step's keys or values
   extern __shared__ __align__(128) unsigned char smem_raw[];
   unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);  // swizzle atoms: 1 KB
   unsigned char* q_s = tiles;
@@ -599,79 +776,81 @@ __global__ void __launch_bounds__(THREADS, BOXES == 1 ? 2 : 1) kernel(const __gr
   __shared__ Plan p;
   __shared__ Barriers bar;
   __shared__ unsigned tmem_base_s;
-  __shared__ float sm_m[GROUPS][128], sm_l[GROUPS][128];
+  __shared__ __align__(16) float sm_max[2][GROUPS][4][ROWS];    // a step's maxima, by the warp of 32 keys (two sets, in turn)
+  __shared__ __align__(16) float sm_shift[SOFT_WARPS][32], sm_fade[SOFT_WARPS][32];
+  __shared__ float sm_m[GROUPS][ROWS], sm_l[GROUPS][4][ROWS];
+  __shared__ float2 sm_ml[ROWS];
   __shared__ int odd_s[GROUPS], skip_s[GROUPS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int hd = a.cache.head_dim, kv = blockIdx.y, per_kv = a.heads / a.cache.kv_heads;
-  pdl_launch_dependents();
   if (tid == 0) {
     for (int s = 0; s < K_STAGES; ++s) { mbar_init(&bar.k_full[s], 1); mbar_init(&bar.k_empty[s], 1); }
     for (int s = 0; s < V_STAGES; ++s) { mbar_init(&bar.v_full[s], 1); mbar_init(&bar.v_empty[s], 1); }
     for (int i = 0; i < GROUPS; ++i) {
       mbar_init(&bar.s_full[i], 1);
-      mbar_init(&bar.s_empty[i], 4);
-      mbar_init(&bar.p_full[i], 4);
+      mbar_init(&bar.s_empty[i], S::GROUP);
+      mbar_init(&bar.p_full[i], S::GROUP);
       mbar_init(&bar.o_full[i], 1);
       odd_s[i] = skip_s[i] = 0;
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_kv) : "memory");
   }
-  if (COPIES > 1)  // (what P never gets a value for is zero)
-    for (int i = tid; i < GROUPS * P_BYTES / 16; i += THREADS) reinterpret_cast<uint4*>(p_s)[i] = make_uint4(0u, 0u, 0u, 0u);
+  // (tensor memory is this block's before the next kernel's blocks may come and ask for theirs)
+  if (warp == SOFT_WARPS + 1) tmem_alloc(&tmem_base_s, S::COLUMNS);
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  pdl_launch_dependents();
   pdl_wait();
-  make_plan(p, a, ROWS);
-  if (p.rows == 0) return;
-  const size_t pair = (size_t)blockIdx.z * gridDim.y + kv;
-  const int begin = (int)((long long)p.total * blockIdx.x / a.splits), end = (int)((long long)p.total * (blockIdx.x + 1) / a.splits);
-  const int steps = end - begin;
-  if (steps > 0 || a.splits == 1) {
-    if (warp == SOFT_WARPS + 1) tmem_alloc(&tmem_base_s, S::COLUMNS);
-    {  // the queries, once a copy; rows beyond the tile and dimensions beyond the head are zeros
-      const bf16* q = static_cast<const bf16*>(a.q);
-      for (int i = tid; i < ROWS * BOXES * 8; i += THREADS) {
-        int r = i / (BOXES * 8), c = i % (BOXES * 8), row = p.row0 + r;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (r < p.rows && c * 8 < hd)
-          v = *reinterpret_cast<const uint4*>(q + ((size_t)(p.token0 + row / per_kv - p.row0 / per_kv) * a.heads + kv * per_kv + row % per_kv) * hd + c * 8);
-#pragma unroll
-        for (int copy = 0; copy < COPIES; ++copy) {
-          int at = copy * ROWS + r;
-          *reinterpret_cast<uint4*>(q_s + (c >> 3) * 16384 + at * 128 + (((c & 7) ^ (at & 7)) << 4)) = v;
-        }
-      }
+  if (warp >= 1 && warp < SOFT_WARPS) {  // (beside the first warp, which makes the plan)
+    // the queries: rows beyond the tile and dimensions beyond the head are zeros; they carry the scale's sign
+    const int first = a.cuts[blockIdx.z / a.tiles], row0 = (int)(blockIdx.z % a.tiles) * ROWS;
+    const int rows = (a.cuts[blockIdx.z / a.tiles + 1] - first) * per_kv - row0;
+    const bf16* q = static_cast<const bf16*>(a.q);
+    for (int i = tid - 32; i < ROWS * BOXES * 8; i += SOFT_WARPS * 32 - 32) {
+      const int r = i / (BOXES * 8), c = i % (BOXES * 8), row = row0 + r;
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (r < rows && c * 8 < hd)
+        v = *reinterpret_cast<const uint4*>(q + ((size_t)(first + row / per_kv) * a.heads + kv * per_kv + row % per_kv) * hd + c * 8);
+      if (a.scale < 0.f) { v.x ^= 0x80008000u; v.y ^= 0x80008000u; v.z ^= 0x80008000u; v.w ^= 0x80008000u; }
+      *reinterpret_cast<uint4*>(q_s + (c >> 3) * (ROWS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    fence_before_sync();
-    __syncthreads();
-    fence_after_sync();
-    const unsigned tmem_s = tmem_base_s, tmem_o = tmem_base_s + GROUPS * 64;
+  }
+  make_plan(p, a, ROWS);
+  const int begin = (int)((long long)p.total * blockIdx.x / a.splits), end = (int)((long long)p.total * (blockIdx.x + 1) / a.splits);
+  const int pages = p.rows ? end - begin : 0, steps = (pages + 1) / 2;
+  float* ex = reinterpret_cast<float*>(k_s);  // at the end: results [GROUPS][ROWS][LD]
+  if (steps > 0) {
+    const unsigned tmem_s = tmem_base_s, tmem_o = tmem_base_s + GROUPS * ROWS;
     if (warp == SOFT_WARPS) {
       int issued_k = 0, issued_v = 0;
       bool ok = true;
-      for (int j0 = 0; j0 < steps && ok; j0 += 32) {
-        int page = 0;
-        if (j0 + lane < steps) {
-          int whose, index = look_up(p, begin + j0 + lane, whose);
-          page = page_of(p, a, whose, index);
-        }
-        for (int u = 0; u < 32 && j0 + u < steps && ok; ++u) {
-          const int j = j0 + u, sk = j % K_STAGES, sv = j % V_STAGES;
-          const int at = __shfl_sync(0xffffffffu, page, u);
+      for (int j0 = 0; j0 < steps && ok; j0 += 16) {
+        const int page = 2 * j0 + lane < pages ? page_at(p, a, begin + 2 * j0 + lane) : 0;
+        for (int u = 0; u < 16 && j0 + u < steps && ok; ++u) {
+          const int j = j0 + u, sk = j % K_STAGES, sv = j % V_STAGES, count = min(2, pages - 2 * j);
+          const int at[2] = {__shfl_sync(0xffffffffu, page, 2 * u), __shfl_sync(0xffffffffu, page, 2 * u + 1)};
           if (lane == 0) {
-            const int row_k = ((at * 2 + 0) * a.cache.kv_heads + kv) * PAGE, row_v = ((at * 2 + 1) * a.cache.kv_heads + kv) * PAGE;
             if (j >= K_STAGES && !mbar_wait(&bar.k_empty[sk], (j / K_STAGES - 1) & 1)) ok = false;
             if (ok) {
-              mbar_expect_tx(&bar.k_full[sk], KV_BYTES);
+              mbar_expect_tx(&bar.k_full[sk], count * (KV_BYTES / 2));
+              for (int c = 0; c < count; ++c)
 #pragma unroll
-              for (int x = 0; x < BOXES; ++x) tma_load_2d(k_s + sk * KV_BYTES + x * 8192, &map_kv, &bar.k_full[sk], x * 64, row_k);
+                for (int x = 0; x < BOXES; ++x)
+                  tma_load_2d(k_s + sk * KV_BYTES + x * BOX + c * (PAGE * 128), &map_kv, &bar.k_full[sk], x * 64,
+                              ((at[c] * 2 + 0) * a.cache.kv_heads + kv) * PAGE);
               issued_k = j + 1;
               if (j >= V_STAGES && !mbar_wait(&bar.v_empty[sv], (j / V_STAGES - 1) & 1)) ok = false;
             }
             if (ok) {
-              mbar_expect_tx(&bar.v_full[sv], KV_BYTES);
+              mbar_expect_tx(&bar.v_full[sv], count * (KV_BYTES / 2));
+              for (int c = 0; c < count; ++c)
 #pragma unroll
-              for (int x = 0; x < BOXES; ++x) tma_load_2d(v_s + sv * KV_BYTES + x * 8192, &map_kv, &bar.v_full[sv], x * 64, row_v);
+                for (int x = 0; x < BOXES; ++x)
+                  tma_load_2d(v_s + sv * KV_BYTES + x * BOX + c * (PAGE * 128), &map_kv, &bar.v_full[sv], x * 64,
+                              ((at[c] * 2 + 1) * a.cache.kv_heads + kv) * PAGE);
               issued_v = j + 1;
             }
           }
@@ -685,28 +864,28 @@ __global__ void __launch_bounds__(THREADS, BOXES == 1 ? 2 : 1) kernel(const __gr
       }
     } else if (warp == SOFT_WARPS + 1) {
       if (lane == 0) {
-        constexpr unsigned idesc = instr_desc(128, 64);
-        const unsigned q_addr = smem_u32(q_s);
-        for (int i = 0; i < steps; ++i) {
+        constexpr unsigned idesc = instr_desc(128, ROWS);
+        const uint64_t q_desc = smem_desc(smem_u32(q_s));
+        bool ok = true;
+        for (int i = 0; i < steps && ok; ++i) {  // (a single last page: the other 64 rows are whatever lies there, and nobody looks)
           const int g = i % GROUPS, s = i % K_STAGES;
-          if (!mbar_wait(&bar.k_full[s], (i / K_STAGES) & 1) || (i >= GROUPS && !mbar_wait(&bar.s_empty[g], (i / GROUPS - 1) & 1))) {
-            *(volatile int*)a.status = 53;
-            break;
-          }
+          ok = mbar_wait(&bar.k_full[s], (i / K_STAGES) & 1) && (i < GROUPS || mbar_wait(&bar.s_empty[g], (i / GROUPS - 1) & 1));
+          if (!ok) break;
           fence_after_sync();
-          const unsigned k_addr = smem_u32(k_s + s * KV_BYTES);
+          const uint64_t k_desc = smem_desc(smem_u32(k_s + s * KV_BYTES));  // (start addresses / 16 are the low bits)
 #pragma unroll
           for (int k = 0; k < BOXES * 4; ++k)
             if (k * 16 < hd)
-              umma(tmem_s + (unsigned)(g * 64), smem_desc(q_addr + (k >> 2) * 16384 + (k & 3) * 32),
-                   smem_desc(k_addr + (k >> 2) * 8192 + (k & 3) * 32), idesc, k > 0 ? 1u : 0u);
+              umma(tmem_s + (unsigned)(g * ROWS), k_desc + (((k >> 2) * BOX + (k & 3) * 32) >> 4),
+                   q_desc + (((k >> 2) * (ROWS * 128) + (k & 3) * 32) >> 4), idesc, k > 0 ? 1u : 0u);
           tcgen05_commit(&bar.k_empty[s]);
           tcgen05_commit(&bar.s_full[g]);
         }
+        if (!ok) *(volatile int*)a.status = 53;
       }
     } else if (warp == SOFT_WARPS + 2) {
       if (lane == 0) {
-        constexpr unsigned idesc = instr_desc(128, 64, true);
+        constexpr unsigned idesc = instr_desc(128, ROWS, true) | (1u << 15);  // both operands' rows are keys
         for (int i = 0; i < steps; ++i) {
           const int g = i % GROUPS, s = i % V_STAGES;
           if (!mbar_wait(&bar.p_full[g], (i / GROUPS) & 1) || !mbar_wait(&bar.v_full[s], (i / V_STAGES) & 1)) {
@@ -715,12 +894,14 @@ __global__ void __launch_bounds__(THREADS, BOXES == 1 ? 2 : 1) kernel(const __gr
           }
           fence_after_sync();
           if (!*(volatile int*)&skip_s[g]) {
-            const unsigned p_addr = smem_u32(p_s + g * P_BYTES), v_addr = smem_u32(v_s + s * KV_BYTES);
+            // (heads of 64: the lower half of the 128 rows comes twice)
+            const uint64_t v_desc = transposed_desc(smem_u32(v_s + s * KV_BYTES), BOXES == 2 ? BOX : 0);
+            const uint64_t p_desc = smem_desc(smem_u32(p_s + g * P_BYTES));
+            const int sixteens = min(8, 4 * (pages - 2 * i));
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-              for (int x = 0; x < BOXES; ++x)
-                umma(tmem_o + (unsigned)(g * S::OUT + x * 64), smem_desc(p_addr + k * 32), smem_desc(v_addr + x * 8192 + k * 2048), idesc,
+            for (int k = 0; k < 8; ++k)
+              if (k < sixteens)
+                umma(tmem_o + (unsigned)(g * ROWS), v_desc + ((k * 2048) >> 4), p_desc + ((k * 2048) >> 4), idesc,
                      (k > 0 || i >= GROUPS) ? 1u : 0u);
           }
           tcgen05_commit(&bar.v_empty[s]);
@@ -728,115 +909,174 @@ __global__ void __launch_bounds__(THREADS, BOXES == 1 ? 2 : 1) kernel(const __gr
         }
       }
     } else {
-      const int g = warp >> 2, r = (warp & 3) * 32 + lane, row = r % ROWS, first_key = r / ROWS * KEYS;
-      const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
-      const unsigned s_addr = tmem_s + lanes + (unsigned)(g * 64 + first_key), o_addr = tmem_o + lanes + (unsigned)(g * S::OUT);
-      unsigned char* p_row = p_s + g * P_BYTES + r * 128;
+      const int g = warp / S::GROUP, half = (warp % S::GROUP) >> 2, quarter = warp & 3;  // 32 keys of the step; 32 of the rows
+      const int key = quarter * 32 + lane, row0 = half * 32, in_group = tid - g * S::GROUP * 32;
+      const unsigned lanes = (unsigned)(quarter * 32) << 16;
+      const unsigned s_addr = tmem_s + lanes + (unsigned)(g * ROWS + row0), o_addr = tmem_o + lanes + (unsigned)(g * ROWS + row0);
+      unsigned char* p_row = p_s + g * P_BYTES + key * 128;
+      // this lane's row of the 32 (every warp of the half keeps the same)
+      const int row = row0 + lane;
       const bool real = row < p.rows;
-      const int token = real ? (p.row0 + row) / per_kv - p.row0 / per_kv : -2;
+      const int token = real ? (p.row0 + row) / per_kv - p.row0 / per_kv : 0;
       const int high = real ? p.position[token] : -1, low = real ? p.low[token] : 0;
-      const float scale = a.scale * 1.4426950408889634f;
-      float m_run = -INFINITY, l_run = 0.f;
+      const float scale = fabsf(a.scale) * 1.4426950408889634f;  // (the queries carry its sign: the largest product is the largest score)
+      const Two scale2 = two(scale, scale);
+      float m_run = -INFINITY;  // of this lane's row
+      Two l[16];                // of all 32 rows, this thread's keys
+#pragma unroll
+      for (int c = 0; c < 16; ++c) l[c] = two(0.f, 0.f);
       bool ok = true;
       int taken = 0;
       // (a wait that ran out is not left at once: the warps of a group meet at barriers that they all have to reach)
       for (int j = g; j < steps; j += GROUPS, ++taken) {
-        int whose;
-        const int at = look_up(p, begin + j, whose) * PAGE;
-        const bool edge = whose >= 0 || at < p.all_from || at + PAGE - 1 > p.all_to;
+        int who0, who1 = EVERYBODY;
+        const int at0 = look_up(p, begin + 2 * j, who0) * PAGE;
+        const bool second = 2 * j + 1 < pages;
+        const int at1 = second ? look_up(p, begin + 2 * j + 1, who1) * PAGE : 0;
+        const bool edge0 = who0 != EVERYBODY || at0 < p.all_from || at0 + PAGE - 1 > p.all_to;
+        const bool edge1 = second && (who1 != EVERYBODY || at1 < p.all_from || at1 + PAGE - 1 > p.all_to);
+        const bool upper = quarter >= 2;  // this warp's page of the two
+        const int position0 = (upper ? at1 : at0) + (quarter & 1) * 32, who = upper ? who1 : who0;  // (of the warp's first key)
+        const bool edge = upper ? edge1 : edge0, none = upper && !second;
         ok = ok && mbar_wait(&bar.s_full[g], (j / GROUPS) & 1);
         __syncwarp();
         fence_after_sync();
-        float v[KEYS];
-#pragma unroll
-        for (int c = 0; c < KEYS; c += 16) tmem_load16_nowait(s_addr + (unsigned)c, reinterpret_cast<unsigned*>(v) + c);
+        float s[32];
+        tmem_load16_nowait(s_addr, reinterpret_cast<unsigned*>(s));
+        tmem_load16_nowait(s_addr + 16u, reinterpret_cast<unsigned*>(s) + 16);
         tmem_wait_ld();
         fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar.s_empty[g]);
-#pragma unroll
-        for (int c = 0; c < KEYS; ++c) v[c] *= scale;
-        unsigned long long seen = ~0ull;
+        unsigned seen = none ? 0u : 0xffffffffu;  // rows that see this thread's key
         if (edge) {
-          const bool mine = whose < 0 || whose == token;
-          seen = 0ull;
+          // a lane's row sees these of the warp's 32 keys; turned round, a lane's key is seen by these of the 32 rows
+          const int last = high - position0, first = low - position0;
+          seen = real && last >= 0 && first < 32 && has_page(p, who, token) ? 0xffffffffu : 0u;
+          if (last < 31) seen &= 0xffffffffu >> (31 - max(last, 0));
+          if (first > 0) seen &= 0xffffffffu << (first & 31);
+          unsigned low_half = 0x0000ffffu;
 #pragma unroll
-          for (int c = 0; c < KEYS; ++c) {
-            const int key = at + first_key + c;
-            const bool sees = mine && key <= high && key >= low;
-            if (sees) seen |= 1ull << c;
-            else v[c] = -INFINITY;
+          for (int o = 16; o > 0; o >>= 1) {
+            const unsigned other = __shfl_xor_sync(0xffffffffu, seen, o);
+            seen = lane & o ? (seen & ~low_half) | (other >> o & low_half) : (seen & low_half) | ((other & low_half) << o);
+            low_half ^= low_half << (o >> 1);
           }
         }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, sum[4] = {0.f, 0.f, 0.f, 0.f};
+        if (edge || none) {
 #pragma unroll
-        for (int c = 0; c < KEYS; ++c) mx[c & 3] = fmaxf(mx[c & 3], v[c]);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          for (int c = 0; c < 32; ++c)
+            if (!(seen >> c & 1u)) s[c] = -INFINITY;
+        }
+        // the rows' maxima over the step
+        float* maxima = &sm_max[taken & 1][g][0][row0];
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          const float4 top = make_float4(largest_of_warp(s[c]), largest_of_warp(s[c + 1]), largest_of_warp(s[c + 2]), largest_of_warp(s[c + 3]));
+          if (lane == 0) *reinterpret_cast<float4*>(&maxima[quarter * ROWS + c]) = top;
+        }
+        asm volatile("bar.sync %0, 128;" ::"r"(2 + g * S::HALVES + half) : "memory");
+        const float largest = fmaxf(fmaxf(maxima[lane], maxima[ROWS + lane]), fmaxf(maxima[2 * ROWS + lane], maxima[3 * ROWS + lane]));
+        const float top = largest > -INFINITY ? largest * scale : -INFINITY;  // (a scale of 0 makes no NaN of it)
         float fade = 1.f;
-        if (top > m_run + 8.f) {  // (also a row's first scores, while its maximum is still -inf)
-          fade = fast_exp2(m_run - top);
+        if (top > m_run) {
+          if (m_run > -INFINITY) fade = fast_exp2(m_run - top);  // (else the row's outputs are zeros so far)
           m_run = top;
         }
-        const float shift = m_run > -INFINITY ? m_run : 0.f;
-        unsigned packed[KEYS / 2];
+        const bool fades = __any_sync(0xffffffffu, fade != 1.f);
+        sm_shift[warp][lane] = m_run > -INFINITY ? -m_run : 0.f;
+        if (fades) sm_fade[warp][lane] = fade;
+        __syncwarp();
+        if (fades) {
 #pragma unroll
-        for (int c = 0; c < KEYS; c += 2) {
-          const float w0 = fast_exp2(v[c] - shift), w1 = fast_exp2(v[c + 1] - shift);
-          sum[c & 3] += w0;
-          sum[(c + 1) & 3] += w1;
-          packed[c / 2] = pack_bf16(w0, w1);
+          for (int c = 0; c < 32; c += 4) {
+            asm volatile("" ::: "memory");  // (what comes next is not fetched ahead: registers)
+            const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(&sm_fade[warp][c]);
+            l[c / 2] = mul2(l[c / 2], f.x);
+            l[c / 2 + 1] = mul2(l[c / 2 + 1], f.y);
+          }
         }
-        l_run = l_run * fade + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
         // the group's previous product has to be over: it reads P and adds to the outputs
         if (taken >= 1) {
-          ok = ok && mbar_wait(&bar.o_full[g], ((j - GROUPS) / GROUPS) & 1);
+          ok = ok && mbar_wait(&bar.o_full[g], (taken - 1) & 1);
           __syncwarp();
           fence_after_sync();
         }
 #pragma unroll
-        for (int c = 0; c < KEYS / 8; ++c)
-          *reinterpret_cast<uint4*>(p_row + (((first_key / 8 + c) ^ (r & 7)) << 4)) =
-              make_uint4(packed[4 * c], packed[4 * c + 1], packed[4 * c + 2], packed[4 * c + 3]);
+        for (int c = 0; c < 32; c += 8) {
+          asm volatile("" ::: "memory");
+          unsigned packed[4];
+#pragma unroll
+          for (int e = 0; e < 8; e += 4) {
+            const ulonglong2 shift = *reinterpret_cast<const ulonglong2*>(&sm_shift[warp][c + e]);
+            const float2 x = apart(fma2(two(s[c + e], s[c + e + 1]), scale2, shift.x));
+            const float2 y = apart(fma2(two(s[c + e + 2], s[c + e + 3]), scale2, shift.y));
+            const float w0 = fast_exp2(x.x), w1 = fast_exp2(x.y), w2 = fast_exp2(y.x), w3 = fast_exp2(y.y);
+            packed[e / 2] = pack_bf16(w0, w1);
+            packed[e / 2 + 1] = pack_bf16(w2, w3);
+            l[(c + e) / 2] = add2(l[(c + e) / 2], two(w0, w1));
+            l[(c + e) / 2 + 1] = add2(l[(c + e) / 2 + 1], two(w2, w3));
+          }
+          *reinterpret_cast<uint4*>(p_row + (((half * 4 + c / 8) ^ (key & 7)) << 4)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+        }
         bool odd = false;
         const unsigned char* v_tile = v_s + (j % V_STAGES) * KV_BYTES;
-        if (edge) {
+        if (edge0 || edge1) {
           ok = ok && mbar_wait(&bar.v_full[j % V_STAGES], (j / V_STAGES) & 1);
+          unsigned bits = 0u;
 #pragma unroll
-          for (int i = 0; i < KV_BYTES / 16 / 128; ++i) {
-            uint4 x = *reinterpret_cast<const uint4*>(v_tile + (i * 128 + r) * 16);
-            odd = odd || odd_pair(x.x) || odd_pair(x.y) || odd_pair(x.z) || odd_pair(x.w);
-          }
-          if (__any_sync(0xffffffffu, odd) && lane == 0) odd_s[g] = 1;
-          asm volatile("bar.sync %0, 128;" ::"r"(2 + g) : "memory");
+          for (int x = 0; x < BOXES; ++x)
+#pragma unroll
+            for (int i = 0; i < BOX / 16 / (S::GROUP * 32); ++i) {
+              const int at = (i * S::GROUP * 32 + in_group) * 16;
+              if (second || at < PAGE * 128) {
+                const uint4 v = *reinterpret_cast<const uint4*>(v_tile + x * BOX + at);
+                bits |= odd_bits(v.x) | odd_bits(v.y) | odd_bits(v.z) | odd_bits(v.w);
+              }
+            }
+          if (__any_sync(0xffffffffu, any_odd(bits)) && lane == 0) odd_s[g] = 1;
+          asm volatile("bar.sync %0, %1;" ::"r"(6 + g), "n"(S::GROUP * 32) : "memory");
           odd = *(volatile int*)&odd_s[g] != 0;
-          asm volatile("bar.sync %0, 128;" ::"r"(2 + g) : "memory");
-          if (r == 0) { odd_s[g] = 0; *(volatile int*)&skip_s[g] = odd; }
-        } else if (r == 0) {
+          asm volatile("bar.sync %0, %1;" ::"r"(6 + g), "n"(S::GROUP * 32) : "memory");
+          if (in_group == 0) { odd_s[g] = 0; *(volatile int*)&skip_s[g] = odd; }
+        } else if (in_group == 0) {
           *(volatile int*)&skip_s[g] = 0;
         }
-        if (odd || (taken >= 1 && __any_sync(0xffffffffu, fade != 1.f))) {
-#pragma unroll 1
-          for (int c = 0; c < S::OUT; c += 16) {
-            unsigned o[16];
-            if (taken >= 1) tmem_load16(o_addr + (unsigned)c, o);
+        if (odd || (taken >= 1 && fades)) {
 #pragma unroll
-            for (int d = 0; d < 16; ++d) o[d] = taken >= 1 ? __float_as_uint(__uint_as_float(o[d]) * fade) : 0u;
+          for (int c0 = 0; c0 < 32; c0 += 16) {
+            unsigned o[16];  // of this thread's dimension, 16 of the rows
+            if (taken >= 1) tmem_load16(o_addr + (unsigned)c0, o);
+#pragma unroll
+            for (int c = 0; c < 16; c += 4) {
+              asm volatile("" ::: "memory");
+              if (taken == 0) o[c] = o[c + 1] = o[c + 2] = o[c + 3] = 0u;
+              if (fades) {
+                const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(&sm_fade[warp][c0 + c]);
+                const float2 x = apart(mul2(two(__uint_as_float(o[c]), __uint_as_float(o[c + 1])), f.x));
+                const float2 y = apart(mul2(two(__uint_as_float(o[c + 2]), __uint_as_float(o[c + 3])), f.y));
+                o[c] = __float_as_uint(x.x); o[c + 1] = __float_as_uint(x.y);
+                o[c + 2] = __float_as_uint(y.x); o[c + 3] = __float_as_uint(y.y);
+              }
+            }
             if (odd) {
+              const int d = quarter * 32 + lane, keys = second ? KEYS : PAGE;  // (heads of 64: dimensions beyond are not used)
 #pragma unroll 1
-              for (int key = 0; key < KEYS; ++key) {
-                if (!(seen >> key & 1ull)) continue;
-                const int at_key = first_key + key;
-                const float w = __bfloat162float(*reinterpret_cast<const bf16*>(p_row + (((at_key >> 3) ^ (r & 7)) << 4) + 2 * (at_key & 7)));
+              for (int k = 0; k < keys; ++k) {
+                const int at_k = (k < PAGE ? at0 : at1) + (k & (PAGE - 1));
+                const unsigned have = __ballot_sync(0xffffffffu, real && has_page(p, k < PAGE ? who0 : who1, token) && at_k <= high && at_k >= low);
+                const float x = __bfloat162float(*reinterpret_cast<const bf16*>(
+                    v_tile + (BOXES == 2 ? d >> 6 : 0) * BOX + k * 128 + ((((d & 63) >> 3) ^ (k & 7)) << 4) + 2 * (d & 7)));
+                const unsigned char* weights = p_s + g * P_BYTES + k * 128;
 #pragma unroll
-                for (int d = 0; d < 16; ++d) {
-                  const int column = (c & 63) + d;
-                  const bf16 x = *reinterpret_cast<const bf16*>(v_tile + (c >> 6) * 8192 + at_key * 128 + (((column >> 3) ^ (at_key & 7)) << 4) + 2 * (column & 7));
-                  o[d] = __float_as_uint(fmaf(w, __bfloat162float(x), __uint_as_float(o[d])));
+                for (int c = 0; c < 16; ++c) {
+                  const int r = row0 + c0 + c;
+                  const float w = __bfloat162float(*reinterpret_cast<const bf16*>(weights + (((r >> 3) ^ (k & 7)) << 4) + 2 * (r & 7)));
+                  if (have >> (c0 + c) & 1u) o[c] = __float_as_uint(fmaf(w, x, __uint_as_float(o[c])));
                 }
               }
-              __syncwarp();
             }
-            tmem_store16(o_addr + (unsigned)c, o);
+            tmem_store16(o_addr + (unsigned)c0, o);
           }
           tmem_wait_st();
           fence_before_sync();
@@ -849,264 +1089,307 @@ __global__ void __launch_bounds__(THREADS, BOXES == 1 ? 2 : 1) kernel(const __gr
       if (!ok) *(volatile int*)a.status = 55;
       __syncwarp();
       fence_after_sync();
-      // ---- groups and copies together: a common maximum, then sums through shared memory (P and the stages are free: every
-      // product has been added)
-      sm_m[g][r] = m_run;
-      sm_l[g][r] = l_run;
-      asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
-      float top = -INFINITY;
+      // ---- the groups together. Lane c ends with row c's sum over the warp's 32 keys: pairs of lanes share their rows out, then fours, ..
+      float sums[32];
 #pragma unroll
-      for (int i = 0; i < GROUPS; ++i)
+      for (int c = 0; c < 16; ++c) {
+        const float2 x = apart(l[c]);
+        sums[2 * c] = x.x;
+        sums[2 * c + 1] = x.y;
+      }
 #pragma unroll
-        for (int copy = 0; copy < COPIES; ++copy) top = fmaxf(top, sm_m[i][copy * ROWS + row]);
-      const float w = m_run > -INFINITY ? fast_exp2(m_run - top) : 0.f;
-      float* ex = reinterpret_cast<float*>(p_s);
-#pragma unroll 1
-      for (int c = 0; c < S::OUT; c += 16) {
-        unsigned o[16];
-        if (taken >= 1) tmem_load16(o_addr + (unsigned)c, o);
+      for (int o = 16; o > 0; o >>= 1) {
+        const bool up = (lane & o) != 0;
 #pragma unroll
-        for (int d = 0; d < 16; d += 4) {
-          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (taken >= 1 && w != 0.f)
-            x = make_float4(__uint_as_float(o[d]) * w, __uint_as_float(o[d + 1]) * w, __uint_as_float(o[d + 2]) * w, __uint_as_float(o[d + 3]) * w);
-          *reinterpret_cast<float4*>(ex + (size_t)(g * 128 + r) * S::LD + c + d) = x;
+        for (int c = 0; c < o; ++c) {
+          const float give = up ? sums[c] : sums[c + o], keep = up ? sums[c + o] : sums[c];
+          sums[c] = keep + __shfl_xor_sync(0xffffffffu, give, o);
         }
       }
+      if (high < 0) m_run = -INFINITY;  // (a row that sees nothing)
+      sm_l[g][quarter][row] = high < 0 ? 0.f : sums[0];
+      if (quarter == 0) sm_m[g][row] = m_run;
       asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
-      const int fours = hd / 4;
-      for (int i = tid; i < p.rows * fours; i += SOFT_WARPS * 32) {
-        const int to = i / fours, d = (i % fours) * 4;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        float most = -INFINITY, total = 0.f;
+      float most = sm_m[0][row];
 #pragma unroll
-        for (int e = 0; e < GROUPS * COPIES; ++e) most = fmaxf(most, sm_m[e / COPIES][e % COPIES * ROWS + to]);
+      for (int i = 1; i < GROUPS; ++i) most = fmaxf(most, sm_m[i][row]);
+      const float w = share_of(m_run, most);
+      const int d = quarter * 32 + lane;
 #pragma unroll
-        for (int e = 0; e < GROUPS * COPIES; ++e) {
-          const int from = e % COPIES * ROWS + to;
-          float4 y = *reinterpret_cast<const float4*>(ex + (size_t)(e / COPIES * 128 + from) * S::LD + d);
-          x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-          const float me = sm_m[e / COPIES][from], le = sm_l[e / COPIES][from];
-          total += me > -INFINITY ? le * fast_exp2(me - most) : le;
+      for (int c0 = 0; c0 < 32; c0 += 16) {
+        unsigned o[16];
+        if (taken >= 1) tmem_load16(o_addr + (unsigned)c0, o);
+        float* to = ex + (size_t)(g * ROWS + row0 + c0) * S::LD + d;
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          const float wc = __shfl_sync(0xffffffffu, w, c0 + c);
+          if (d < BOXES * 64) to[c * S::LD] = taken >= 1 && wc != 0.f ? __uint_as_float(o[c]) * wc : 0.f;
         }
-        if (a.splits == 1) {
-          const float inv = total != 0.f ? 1.f / total : 0.f;
-          const int in_group = p.row0 + to, t = p.token0 + in_group / per_kv - p.row0 / per_kv;
-          *reinterpret_cast<uint2*>(static_cast<bf16*>(a.out) + ((size_t)t * a.heads + kv * per_kv + in_group % per_kv) * hd + d) =
-              make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
-        } else {
-          *reinterpret_cast<float4*>(a.scratch + ((pair * a.splits + blockIdx.x) * ROWS + to) * hd + d) = x;
-          if (d == 0) {
-            float* ml = a.scratch + (size_t)gridDim.z * gridDim.y * a.splits * ROWS * hd + ((pair * a.splits + blockIdx.x) * ROWS + to) * 2;
-            *reinterpret_cast<float2*>(ml) = make_float2(most, total);
-          }
+      }
+      if (g == 0 && quarter == 0) {
+        float total = 0.f;
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+          const float part = (sm_l[i][0][row] + sm_l[i][1][row]) + (sm_l[i][2][row] + sm_l[i][3][row]);
+          total += sm_m[i][row] > -INFINITY ? part * share_of(sm_m[i][row], most) : part;
         }
+        sm_ml[row] = make_float2(most, total);
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
+      for (int i = tid; i < ROWS * (BOXES * 16); i += SOFT_WARPS * 32) {  // (into the first group's place)
+        float4* x = reinterpret_cast<float4*>(ex + (size_t)(i / (BOXES * 16)) * S::LD + (i % (BOXES * 16)) * 4);
+        float4 z = *x;
+#pragma unroll
+        for (int e = 1; e < GROUPS; ++e) {
+          const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(x) + (size_t)e * ROWS * S::LD);
+          z.x += y.x; z.y += y.y; z.z += y.z; z.w += y.w;
+        }
+        *x = z;
       }
     }
     fence_before_sync();
-    __syncthreads();
-    if (warp == SOFT_WARPS + 1) tmem_dealloc(tmem_base_s, S::COLUMNS);
+  } else {
+    for (int r = tid; r < ROWS; r += S::THREADS) sm_ml[r] = make_float2(-INFINITY, 0.f);
   }
-  if (a.splits == 1) return;
-  if (is_last(p, a, pair)) join<bf16, ROWS, THREADS>(p, a, pair, reinterpret_cast<float*>(tiles));
+  __syncthreads();
+  if (warp == SOFT_WARPS + 1) tmem_dealloc(tmem_base_s, S::COLUMNS);
+  if (p.rows == 0) return;
+  finish<bf16, ROWS>(p, a, ex, S::LD, sm_ml, reinterpret_cast<float*>(q_s));
 }
 
-template <int BOXES, int COPIES>
+template <int BOXES, int ROWS>
 int launch(const Args& a, long long pages, dim3 grid, cudaStream_t stream) {
-  typedef Shape<BOXES> S;
-  static_assert((MAX_SPLITS + 1) * 128 * 4 + 1024 <= S::SMEM, "the weights of the join");
+  typedef Shape<BOXES, ROWS> S;
+  static_assert(MAX_CLUSTERS * ROWS * 8 + 1024 <= S::SMEM, "what the join keeps");
   CUtensorMap map;
   if (!make_map(&map, a.cache.base, pages * 2 * a.cache.kv_heads * PAGE, a.cache.head_dim, PAGE)) return DLLM_LAUNCH_FAILED;
   static std::atomic<unsigned long long> done{0};
-  if (!dllm_allow_shared((const void*)kernel<BOXES, COPIES>, S::SMEM, done)) return DLLM_LAUNCH_FAILED;
-  return dllm_launch_pdl(kernel<BOXES, COPIES>, grid, dim3(THREADS), S::SMEM, stream, map, a);
+  if (!dllm_allow_shared((const void*)kernel<BOXES, ROWS>, S::SMEM, done)) return DLLM_LAUNCH_FAILED;
+  return launch_clusters(kernel<BOXES, ROWS>, grid, S::THREADS, S::SMEM, a.cluster, stream, map, a);
 }
 }  // namespace t5
 
 // ---- everything else ---------------------------------------------------------------------------------------------
-// 16 query rows a tile, 128 threads. A page's keys, then its values, lie in shared memory as float32. Scores: a thread has one
-// key and half of the rows; the softmax: a warp four rows; the sums: a thread four dimensions and some of the rows.
-constexpr int FMA_ROWS = 16, FMA_THREADS = 128, FMA_DIM = 256;
+// 16 query rows a tile, 256 threads, pages by cp.async into a ring of one or two stages, in the cache's type. Scores: a thread has one of
+// a page's 64 keys and four rows. The rows' maxima go through shared memory, the weights of a key's 16 rows lie side by side in
+// it. Sums: a thread has four dimensions and four rows, and every n-th key; the n groups are added at the end.
+constexpr int FMA_ROWS = 16, FMA_THREADS = 256, FMA_DIM = 256, FMA_LD = 20;
+constexpr int FMA_MOST = 152 << 10;  // bytes of dynamic shared memory: heads of 128 in float32, two stages; of 256, one
+
+__device__ __forceinline__ float4 four(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 four(const bf16* p) {
+  const uint2 raw = *reinterpret_cast<const uint2*>(p);
+  const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x));
+  const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+template <typename T> __host__ __device__ constexpr int fma_row(int hd) { return hd + 16 / (int)sizeof(T); }  // a page's row in shared memory
+template <typename T> __host__ __device__ constexpr int fma_stages(int hd) { return hd * (int)sizeof(T) <= 512 ? 2 : 1; }
 
 template <typename T>
 __global__ void __launch_bounds__(FMA_THREADS) fma_kernel(const Args a) {
   extern __shared__ __align__(128) unsigned char smem_raw[];
   __shared__ Plan p;
-  __shared__ float sm_p[FMA_ROWS][PAGE + 1], sm_m[FMA_ROWS], sm_l[FMA_ROWS], sm_fade[FMA_ROWS];
-  __shared__ int row_token[FMA_ROWS];
+  __shared__ Stretch list;
+  __shared__ __align__(16) float sm_p[PAGE * FMA_LD];
+  __shared__ float sm_max[2][2][FMA_ROWS], sm_fade[FMA_ROWS], sm_l[2][FMA_ROWS];
+  __shared__ float2 sm_ml[FMA_ROWS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int hd = a.cache.head_dim, kv = blockIdx.y, per_kv = a.heads / a.cache.kv_heads, ld = hd + 4;
-  float* q_s = reinterpret_cast<float*>(smem_raw);  // [FMA_ROWS][ld]
-  float* tile = q_s + FMA_ROWS * ld;                 // [PAGE][ld]
+  const int hd = a.cache.head_dim, kv = blockIdx.y, per_kv = a.heads / a.cache.kv_heads;
+  const int ld = hd + 4, row = fma_row<T>(hd), stages = fma_stages<T>(hd), fours = hd / 4;
+  float* q_s = reinterpret_cast<float*>(smem_raw);             // [FMA_ROWS][ld]; at the end the sums
+  T* ring = reinterpret_cast<T*>(q_s + FMA_ROWS * ld);         // per stage: keys, values [PAGE][row]
+  float* groups_s = q_s + FMA_ROWS * ld;                       // at the end: [groups][FMA_ROWS][ld]
   pdl_launch_dependents();
   pdl_wait();
-  make_plan(p, a, FMA_ROWS);
-  if (p.rows == 0) return;
-  const size_t pair = (size_t)blockIdx.z * gridDim.y + kv;
-  const int begin = (int)((long long)p.total * blockIdx.x / a.splits), end = (int)((long long)p.total * (blockIdx.x + 1) / a.splits);
-  const int fours = hd / 4;
-  if (begin < end || a.splits == 1) {
-    for (int i = tid; i < FMA_ROWS * hd; i += FMA_THREADS) {
-      int r = i / hd, d = i % hd, row = p.row0 + r;
-      float v = 0.f;
-      if (r < p.rows)
-        v = to_float(static_cast<const T*>(a.q)[((size_t)(p.token0 + row / per_kv - p.row0 / per_kv) * a.heads + kv * per_kv + row % per_kv) * hd + d]);
-      q_s[r * ld + d] = v;
-    }
-    if (tid < FMA_ROWS) {
-      sm_m[tid] = -INFINITY;
-      sm_l[tid] = 0.f;
-      row_token[tid] = tid < p.rows ? (p.row0 + tid) / per_kv - p.row0 / per_kv : -2;
-    }
-    // sums: this thread's four dimensions (of up to 64) and rows: tid / fours, then in steps
-    const int columns = min(fours, FMA_THREADS), step = FMA_THREADS / columns;
-    const int d4 = (tid % columns) * 4, r_first = tid / columns;
-    const bool sums = r_first < step;
-    float4 acc[FMA_ROWS];  // (rows r_first + step * i)
-#pragma unroll
-    for (int i = 0; i < FMA_ROWS; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    const float scale = a.scale * 1.4426950408889634f;
-    const T* base = static_cast<const T*>(a.cache.base);
-    __syncthreads();
-    for (int part = begin; part < end; part += LIST) {
-      const int count = min(LIST, end - part);
-      list_pages(p, a, part, part + count);
-      for (int it = 0; it < count; ++it) {
-        const int whose = p.whose[it], at = p.at[it];
-        auto fetch = [&](int which) {
-          const T* src = base + kv_offset(a.cache, p.page[it], which, kv, 0);
-          int from = whose < 0 ? 0 : p.low[whose], to = whose < 0 ? p.position[p.longest] : p.position[whose];
-          for (int i = tid; i < PAGE * fours; i += FMA_THREADS) {
-            int r = i / fours, d = (i % fours) * 4;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (at + r >= from && at + r <= to) {
-              const T* s = src + (size_t)r * hd + d;
-              v = make_float4(to_float(s[0]), to_float(s[1]), to_float(s[2]), to_float(s[3]));
-            }
-            *reinterpret_cast<float4*>(tile + r * ld + d) = v;
-          }
-        };
-        fetch(0);
-        __syncthreads();
-        {
-          const int key = tid & 63, half = tid >> 6;
-          float dot[FMA_ROWS / 2];
-#pragma unroll
-          for (int i = 0; i < FMA_ROWS / 2; ++i) dot[i] = 0.f;
-          for (int d = 0; d < hd; d += 4) {
-            float4 k4 = *reinterpret_cast<const float4*>(tile + key * ld + d);
-#pragma unroll
-            for (int i = 0; i < FMA_ROWS / 2; ++i) {
-              float4 q4 = *reinterpret_cast<const float4*>(q_s + (half * (FMA_ROWS / 2) + i) * ld + d);
-              dot[i] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, dot[i]))));
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < FMA_ROWS / 2; ++i) {
-            int r = half * (FMA_ROWS / 2) + i, t = row_token[r];
-            bool sees = t >= 0 && (whose < 0 || whose == t) && at + key <= p.position[t] && at + key >= p.low[t];
-            sm_p[r][key] = sees ? dot[i] * scale : -INFINITY;
-          }
-        }
-        __syncthreads();
-        fetch(1);
-        for (int r = warp; r < FMA_ROWS; r += FMA_THREADS / 32) {
-          float x0 = sm_p[r][lane], x1 = sm_p[r][lane + 32];
-          float top = fmaxf(warp_max(fmaxf(x0, x1)), sm_m[r]);
-          float shift = top > -INFINITY ? top : 0.f;
-          // (a masked key's weight is marked by -1: its value is not multiplied)
-          float w0 = x0 == -INFINITY ? 0.f : exp2f(x0 - shift), w1 = x1 == -INFINITY ? 0.f : exp2f(x1 - shift);
-          float sum = warp_sum(w0 + w1);
-          sm_p[r][lane] = x0 == -INFINITY ? -1.f : w0;
-          sm_p[r][lane + 32] = x1 == -INFINITY ? -1.f : w1;
-          if (lane == 0) {
-            float fade = sm_m[r] > -INFINITY ? exp2f(sm_m[r] - shift) : 0.f;
-            sm_fade[r] = fade;
-            sm_l[r] = sm_l[r] * fade + sum;
-            sm_m[r] = top;
-          }
-        }
-        __syncthreads();
-        if (sums) {
-#pragma unroll
-          for (int i = 0; i < FMA_ROWS; ++i) {
-            int r = r_first + step * i;
-            if (r < FMA_ROWS) {
-              float f = sm_fade[r];
-              acc[i].x *= f; acc[i].y *= f; acc[i].z *= f; acc[i].w *= f;
-            }
-          }
-          for (int key = 0; key < PAGE; ++key) {
-            float4 v = *reinterpret_cast<const float4*>(tile + key * ld + d4);
-#pragma unroll
-            for (int i = 0; i < FMA_ROWS; ++i) {
-              int r = r_first + step * i;
-              if (r < FMA_ROWS) {
-                float w = sm_p[r][key];
-                if (w != -1.f) {
-                  acc[i].x = fmaf(w, v.x, acc[i].x);
-                  acc[i].y = fmaf(w, v.y, acc[i].y);
-                  acc[i].z = fmaf(w, v.z, acc[i].z);
-                  acc[i].w = fmaf(w, v.w, acc[i].w);
-                }
-              }
-            }
-          }
-        }
-        __syncthreads();
-      }
-    }
-    if (sums) {
-#pragma unroll
-      for (int i = 0; i < FMA_ROWS; ++i) {
-        int r = r_first + step * i;
-        if (r < FMA_ROWS && r < p.rows) {
-          if (a.splits == 1) {
-            float inv = sm_l[r] != 0.f ? 1.f / sm_l[r] : 0.f;
-            int row = p.row0 + r, t = p.token0 + row_token[r];
-            T* to = static_cast<T*>(a.out) + ((size_t)t * a.heads + kv * per_kv + row % per_kv) * hd + d4;
-            to[0] = from_float<T>(acc[i].x * inv);
-            to[1] = from_float<T>(acc[i].y * inv);
-            to[2] = from_float<T>(acc[i].z * inv);
-            to[3] = from_float<T>(acc[i].w * inv);
-          } else {
-            *reinterpret_cast<float4*>(a.scratch + ((pair * a.splits + blockIdx.x) * FMA_ROWS + r) * hd + d4) = acc[i];
-          }
-        }
-      }
-    }
-    if (a.splits > 1 && tid < p.rows) {
-      float* ml = a.scratch + (size_t)gridDim.z * gridDim.y * a.splits * FMA_ROWS * hd + ((pair * a.splits + blockIdx.x) * FMA_ROWS + tid) * 2;
-      *reinterpret_cast<float2*>(ml) = make_float2(sm_m[tid], sm_l[tid]);
+  if (warp >= 1) {  // (beside the first warp, which makes the plan)
+    const int first = a.cuts[blockIdx.z / a.tiles], row0 = (int)(blockIdx.z % a.tiles) * FMA_ROWS;
+    const int rows = (a.cuts[blockIdx.z / a.tiles + 1] - first) * per_kv - row0;
+    for (int i = tid - 32; i < FMA_ROWS * fours; i += FMA_THREADS - 32) {
+      const int r = i / fours, d = (i % fours) * 4, at = row0 + r;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < rows) v = four(static_cast<const T*>(a.q) + ((size_t)(first + at / per_kv) * a.heads + kv * per_kv + at % per_kv) * hd + d);
+      *reinterpret_cast<float4*>(q_s + r * ld + d) = v;
     }
   }
-  if (a.splits == 1) return;
-  if (is_last(p, a, pair)) join<T, FMA_ROWS, FMA_THREADS>(p, a, pair, reinterpret_cast<float*>(smem_raw));
+  make_plan(p, a, FMA_ROWS);
+  if (p.rows == 0) return;
+  const int begin = (int)((long long)p.total * blockIdx.x / a.splits), end = (int)((long long)p.total * (blockIdx.x + 1) / a.splits);
+  if (begin < end) {
+    const T* base = static_cast<const T*>(a.cache.base);
+    const float scale = a.scale * 1.4426950408889634f;
+    // scores: this thread's key and rows
+    const int key = (warp >> 2) * 32 + lane, r0 = (warp & 3) * 4;
+    int token[4], high[4], low[4];
+    float m[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool real = r0 + i < p.rows;
+      token[i] = real ? (p.row0 + r0 + i) / per_kv - p.row0 / per_kv : -1;
+      high[i] = real ? p.position[token[i]] : -1;
+      low[i] = real ? p.low[token[i]] : 0;
+      m[i] = -INFINITY;
+      l[i] = 0.f;
+    }
+    // sums: this thread's dimensions, rows and keys
+    const int each = fours * 4, n_groups = min(16, FMA_THREADS / each), group = tid / each;
+    const int d4 = (tid % each) % fours * 4, s0 = (tid % each) / fours * 4;
+    float4 acc[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int chunks = hd * (int)sizeof(T) / 16;
+    for (int part = begin; part < end; part += LIST) {
+      const int count = min(LIST, end - part);
+      fill(list, p, a, part, part + count);
+      auto bring = [&](int i) {
+        const T* keys = base + kv_offset(a.cache, list.page[i], 0, kv, 0);
+        const size_t values = (size_t)a.cache.kv_heads * PAGE * hd;
+        T* to = ring + (size_t)(i % stages) * 2 * PAGE * row;
+        for (int c = tid; c < PAGE * chunks; c += FMA_THREADS) {
+          const int r = c / chunks, d = c % chunks * (16 / (int)sizeof(T));
+          cp_async_16(to + r * row + d, keys + r * hd + d, true);
+          cp_async_16(to + (PAGE + r) * row + d, keys + values + r * hd + d, true);
+        }
+      };
+      bring(0);
+      cp_async_commit();
+      for (int it = 0; it < count; ++it) {
+        if (stages > 1) {
+          if (it + 1 < count) bring(it + 1);
+          cp_async_commit();
+          cp_async_wait<1>();
+        } else {
+          cp_async_wait<0>();
+        }
+        __syncthreads();
+        const T* keys = ring + (size_t)(it % stages) * 2 * PAGE * row;
+        const T* vals = keys + PAGE * row;
+        const int who = list.who[it], at = list.at[it];
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int d = 0; d < hd; d += 4) {
+          const float4 k4 = four(keys + key * row + d);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float4 q4 = four(q_s + (r0 + i) * ld + d);
+            s[i] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[i]))));
+          }
+        }
+        bool sees[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sees[i] = token[i] >= 0 && at + key <= high[i] && at + key >= low[i] && has_page(p, who, token[i]);
+          s[i] = sees[i] ? s[i] * scale : -INFINITY;
+          const float top = warp_max(s[i]);
+          if (lane == 0) sm_max[it & 1][warp >> 2][r0 + i] = top;
+        }
+        __syncthreads();
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float top = fmaxf(m[i], fmaxf(sm_max[it & 1][0][r0 + i], sm_max[it & 1][1][r0 + i]));
+          const float shift = top > -INFINITY ? top : 0.f;
+          const float fade = m[i] > -INFINITY ? exp2f(m[i] - shift) : 1.f;
+          m[i] = top;
+          // (a masked key's weight is marked by -1: its value is not multiplied)
+          w[i] = sees[i] ? exp2f(s[i] - shift) : -1.f;
+          l[i] = l[i] * fade + (sees[i] ? w[i] : 0.f);
+          if (key == 0) sm_fade[r0 + i] = fade;
+        }
+        *reinterpret_cast<float4*>(sm_p + key * FMA_LD + r0) = make_float4(w[0], w[1], w[2], w[3]);
+        __syncthreads();
+        if (group < n_groups) {
+          const float4 f = four(sm_fade + s0);
+          const float fades[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            acc[i].x *= fades[i]; acc[i].y *= fades[i]; acc[i].z *= fades[i]; acc[i].w *= fades[i];
+          }
+          for (int k = group; k < PAGE; k += n_groups) {
+            const float4 v = four(vals + k * row + d4), weights = four(sm_p + k * FMA_LD + s0);
+            const float each_w[4] = {weights.x, weights.y, weights.z, weights.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (each_w[i] != -1.f) {
+                acc[i].x = fmaf(each_w[i], v.x, acc[i].x);
+                acc[i].y = fmaf(each_w[i], v.y, acc[i].y);
+                acc[i].z = fmaf(each_w[i], v.z, acc[i].z);
+                acc[i].w = fmaf(each_w[i], v.w, acc[i].w);
+              }
+          }
+        }
+        __syncthreads();
+        if (stages == 1) {
+          if (it + 1 < count) bring(it + 1);
+          cp_async_commit();
+        }
+      }
+      cp_async_wait<0>();
+      __syncthreads();
+    }
+    // the groups of keys together, in order; sums over a row's keys
+    if (group < n_groups)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(groups_s + (size_t)(group * FMA_ROWS + s0 + i) * ld + d4) = acc[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float sum = warp_sum(l[i]);
+      if (lane == 0) sm_l[warp >> 2][r0 + i] = sum;
+    }
+    __syncthreads();
+    for (int i = tid; i < FMA_ROWS * fours; i += FMA_THREADS) {
+      const int r = i / fours, d = (i % fours) * 4;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int g = 0; g < n_groups; ++g) {
+        const float4 y = four(groups_s + (size_t)(g * FMA_ROWS + r) * ld + d);
+        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+      }
+      *reinterpret_cast<float4*>(q_s + r * ld + d) = x;
+    }
+    if (lane == 0 && warp < 4)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sm_ml[r0 + i] = make_float2(m[i], sm_l[0][r0 + i] + sm_l[1][r0 + i]);
+  } else {
+    if (tid < FMA_ROWS) sm_ml[tid] = make_float2(-INFINITY, 0.f);
+  }
+  finish<T, FMA_ROWS>(p, a, q_s, ld, sm_ml, groups_s);
 }
 
 // ---- launch shapes -------------------------------------------------------------------------------------------------
-enum { FMA = 0, MMA = 1, TCGEN05 = 2 };
-struct Shape { int kind, rows, tiles, splits; };
+enum { FMA, MMA, TCGEN05 };
+struct Shape { int kind, rows, tiles, splits, cluster; };
 
-// `kind`: -1 chooses.
-Shape shape_of(int kind, int dtype, int heads, int kv_heads, int head_dim, int groups, int max_rows, int max_context) {
+Shape shape_of(int dtype, int heads, int kv_heads, int head_dim, int groups, int max_rows, int max_context) {
   Shape s;
-  const int query_rows = max_rows * (heads / kv_heads);
-  const bool mma = dtype == DLLM_BF16 && head_dim % 16 == 0 && head_dim <= 128, tcgen05 = mma && head_dim >= 64;
-  const int pages = (max_context + PAGE - 1) / PAGE;
-  s.kind = kind >= 0 ? kind : tcgen05 && pages > 4 ? TCGEN05 : mma ? MMA : FMA;
-  if ((s.kind == TCGEN05 && !tcgen05) || (s.kind == MMA && !mma)) s.kind = FMA;
+  const int query_rows = max_rows * (heads / kv_heads), pages = (max_context + PAGE - 1) / PAGE;
+  const bool tensor = dtype == DLLM_BF16 && head_dim % 16 == 0 && head_dim <= 128;
+  // (tcgen05 against mma.sync with heads of 64 and 128, us: 1 x 4 beams on 110 positions, 9 heads on 3, 9.3 and 8.9; eight new tokens, 32
+  // heads on 8, on 2,000 positions 10.5 and 14.4, 10.7 and 19.5, on 80,000 41 and 84, 61 and 129)
+  s.kind = !tensor ? FMA : head_dim >= 64 ? TCGEN05 : MMA;
   if (s.kind == FMA) s.rows = FMA_ROWS;
   else if (s.kind == MMA) s.rows = query_rows <= 16 ? 16 : query_rows <= 32 ? 32 : 64;
-  else s.rows = query_rows <= 32 ? 32 : query_rows <= 64 ? 64 : 128;
+  else s.rows = query_rows <= 32 ? 32 : 64;
   s.tiles = (query_rows + s.rows - 1) / s.rows;
-  // as many splits as the device has places for, but not more than there can be pages
-  const long long pairs = (long long)groups * s.tiles * kv_heads;
-  const long long places = 148LL * (s.kind == TCGEN05 && head_dim > 64 ? 1 : 2);
-  long long splits = places / (pairs > 0 ? pairs : 1);
-  if (splits > pages + max_rows) splits = pages + max_rows;
-  if (splits > MAX_SPLITS) splits = MAX_SPLITS;
-  s.splits = splits < 1 ? 1 : (int)splits;
+  // Blocks of a tile and kv head: as many as fill the device, but not more than there can be pages, in the largest clusters that
+  // do not cost more than an eighth of them; where there are at most 64 pages one cluster, which needs no scratch and no second
+  // round. (Clusters of 1, 2, 4 and 8 blocks that are resident at a time: a cluster lies within a part of the device, and eighths
+  // of a part are left over.) Eight new tokens, 32 heads on 8 of 128, us with one cluster of 8, 4 of 4, 9 of 2 and 18 of 1: 2,000 positions
+  // 13.4, 17.2, 20.7, 24.1; 80,000: -, 62.6, 65.9, 70.1.
+  static const int RESIDENT[2][4] = {{148, 74, 33, 15}, {296, 148, 71, 33}};
+  const int several = s.kind == MMA || (s.kind == FMA && head_dim * (dtype == DLLM_BF16 ? 2 : 4) <= 256);  // (two of a multiprocessor)
+  const long long pairs = (long long)groups * s.tiles * kv_heads, most = pages + max_rows;
+  long long blocks[4], best = 0;
+  for (int c = 0; c < 4; ++c) {
+    long long n = RESIDENT[several][c] / pairs;
+    if (n > MAX_CLUSTERS) n = MAX_CLUSTERS;
+    if (pages <= 64 && n > 1 && c > 0) n = 1;
+    if (pages <= 64 && n > 1) n = 0;
+    if (n << c > most) n = most >> c;
+    blocks[c] = n << c;
+    if (blocks[c] > best) best = blocks[c];
+  }
+  s.splits = s.cluster = 1;
+  for (int c = 0; c < 4; ++c)
+    if (blocks[c] > 0 && blocks[c] * 8 >= best * 7) { s.cluster = 1 << c; s.splits = (int)blocks[c]; }
   return s;
 }
 
@@ -1114,36 +1397,40 @@ template <int HD, int MT, int WM, int STAGES>
 int launch_mma(const Args& a, dim3 grid, cudaStream_t stream) {
   constexpr int ROWS = 16 * MT * WM;
   constexpr int ring = STAGES * 2 * 64 * HD * 2, sums = 4 * ROWS * HD * 4;
-  constexpr int weights = (MAX_SPLITS + 1) * ROWS * 4;
+  constexpr int weights = MAX_CLUSTERS * ROWS * 8;
   constexpr int bytes = ROWS * HD * 2 + (ring > sums ? ring : sums);
   constexpr int smem = bytes > weights ? bytes : weights;
   static std::atomic<unsigned long long> done{0};
   if (!dllm_allow_shared((const void*)mma_kernel<HD, MT, WM, STAGES>, smem, done)) return DLLM_LAUNCH_FAILED;
-  return dllm_launch_pdl(mma_kernel<HD, MT, WM, STAGES>, grid, dim3(WM * 128), smem, stream, a);
+  return launch_clusters(mma_kernel<HD, MT, WM, STAGES>, grid, WM * 128, smem, a.cluster, stream, a);
 }
 
 template <typename T>
 int launch_fma(const Args& a, dim3 grid, cudaStream_t stream) {
-  const int tiles = (FMA_ROWS + PAGE) * (a.cache.head_dim + 4) * 4, weights = (a.splits + 1) * FMA_ROWS * 4;
+  const int hd = a.cache.head_dim, rows = FMA_ROWS * (hd + 4) * 4;
+  const int ring = fma_stages<T>(hd) * 2 * PAGE * fma_row<T>(hd) * (int)sizeof(T);
+  const int each = hd, n = FMA_THREADS / each < 16 ? FMA_THREADS / each : 16;  // (groups of keys, of hd / 4 x 4 threads)
+  const int sums = n * FMA_ROWS * (hd + 4) * 4, weights = MAX_CLUSTERS * FMA_ROWS * 8;
+  const int most = ring > sums ? ring : sums;
   static std::atomic<unsigned long long> done{0};
-  if (!dllm_allow_shared((const void*)fma_kernel<T>, (FMA_ROWS + PAGE) * (FMA_DIM + 4) * 4, done)) return DLLM_LAUNCH_FAILED;
-  return dllm_launch_pdl(fma_kernel<T>, grid, dim3(FMA_THREADS), tiles > weights ? tiles : weights, stream, a);
+  if (!dllm_allow_shared((const void*)fma_kernel<T>, FMA_MOST, done)) return DLLM_LAUNCH_FAILED;
+  return launch_clusters(fma_kernel<T>, grid, FMA_THREADS, rows + (most > weights ? most : weights), a.cluster, stream, a);
 }
 }  // namespace
 
-// Query rows of a tile in the low 16 bits, splits above: scratch holds groups x tiles x kv_heads x splits x rows x
-// (head_dim + 2) floats, tickets groups x tiles x kv_heads words. kind: -1, or 0, 1, 2 (fused multiply-adds, mma.sync, tcgen05).
-DLLM_EXPORT int dllm_attention_shared_shape(int kind, int dtype, int heads, int kv_heads, int head_dim, int groups, int max_rows,
+// Query rows of a tile in the low 16 bits, clusters above: scratch holds groups x tiles x kv_heads x clusters x rows x
+// (head_dim + 2) floats where there is more than one, tickets groups x tiles x kv_heads words.
+DLLM_EXPORT int dllm_attention_shared_shape(int dtype, int heads, int kv_heads, int head_dim, int groups, int max_rows,
                                             int max_context) {
   if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || groups <= 0 || max_rows <= 0 || max_context <= 0) return DLLM_BAD_ARGUMENT;
-  Shape s = shape_of(kind, dtype, heads, kv_heads, head_dim, groups, max_rows, max_context);
-  return s.rows | s.splits << 16;
+  Shape s = shape_of(dtype, heads, kv_heads, head_dim, groups, max_rows, max_context);
+  return s.rows | s.splits / s.cluster << 16;
 }
 
 // See the head of the file. out, q [tokens, heads * head_dim] in the cache's type; slots, positions: each token's table row and
 // position; cuts [groups + 1]: the groups' first tokens; shared [groups]: pages from the first on that a group's table rows have
 // in common; the cache entry has `pages` pages.
-DLLM_EXPORT int dllm_attention_shared(int kind, void* out, const void* q, void* base, long long pages, const int* page_table,
+DLLM_EXPORT int dllm_attention_shared(void* out, const void* q, void* base, long long pages, const int* page_table,
                                       int max_pages, int page_size, int dtype, int heads, int kv_heads, int head_dim,
                                       const int* slots, const int* positions, const int* cuts, const int* shared, int groups,
                                       int max_rows, int max_context, float scale, int window, float* scratch, unsigned* tickets,
@@ -1153,34 +1440,23 @@ DLLM_EXPORT int dllm_attention_shared(int kind, void* out, const void* q, void* 
   if (head_dim % 8 || head_dim <= 0 || head_dim > FMA_DIM || page_size != PAGE || kv_heads > 65535 ||
       ((uintptr_t)out | (uintptr_t)q | (uintptr_t)base) & 15)
     return DLLM_UNSUPPORTED_SIZE;
-  Shape s = shape_of(kind, dtype, heads, kv_heads, head_dim, groups, max_rows, max_context);
+  Shape s = shape_of(dtype, heads, kv_heads, head_dim, groups, max_rows, max_context);
   if ((long long)groups * s.tiles > 65535) return DLLM_UNSUPPORTED_SIZE;
   Args a{out, q, KvLayout{base, page_table, max_pages, page_size, kv_heads, head_dim}, slots, positions, cuts, shared, scratch,
-         tickets, status, heads, window, s.tiles, s.splits, scale};
+         tickets, status, heads, window, s.tiles, s.splits, s.cluster, scale};
   dim3 grid(s.splits, kv_heads, groups * s.tiles);
   if (s.kind == FMA) return dtype == DLLM_BF16 ? launch_fma<bf16>(a, grid, stream) : launch_fma<float>(a, grid, stream);
   if (s.kind == TCGEN05) {
-    if (pages * 2 * kv_heads * PAGE > 0x7fffffffll) return DLLM_UNSUPPORTED_SIZE;
-    if (head_dim <= 64) {
-      if (s.rows == 32) return t5::launch<1, 4>(a, pages, grid, stream);
-      if (s.rows == 64) return t5::launch<1, 2>(a, pages, grid, stream);
-      return t5::launch<1, 1>(a, pages, grid, stream);
-    }
-    if (s.rows == 32) return t5::launch<2, 4>(a, pages, grid, stream);
-    if (s.rows == 64) return t5::launch<2, 2>(a, pages, grid, stream);
-    return t5::launch<2, 1>(a, pages, grid, stream);
+    if (pages * 2 * kv_heads * PAGE > 0x7fffffffll) return DLLM_UNSUPPORTED_SIZE;  // (a TMA coordinate is an int)
+    if (head_dim == 64) return s.rows == 32 ? t5::launch<1, 32>(a, pages, grid, stream) : t5::launch<1, 64>(a, pages, grid, stream);
+    return s.rows == 32 ? t5::launch<2, 32>(a, pages, grid, stream) : t5::launch<2, 64>(a, pages, grid, stream);
   }
   if (head_dim <= 32) {
     if (s.rows == 16) return launch_mma<32, 1, 1, 4>(a, grid, stream);
     if (s.rows == 32) return launch_mma<32, 2, 1, 4>(a, grid, stream);
     return launch_mma<32, 2, 2, 4>(a, grid, stream);
   }
-  if (head_dim <= 64) {
-    if (s.rows == 16) return launch_mma<64, 1, 1, 4>(a, grid, stream);
-    if (s.rows == 32) return launch_mma<64, 2, 1, 4>(a, grid, stream);
-    return launch_mma<64, 2, 2, 4>(a, grid, stream);
-  }
-  if (s.rows == 16) return launch_mma<128, 1, 1, 3>(a, grid, stream);
-  if (s.rows == 32) return launch_mma<128, 2, 1, 3>(a, grid, stream);
-  return launch_mma<128, 2, 2, 4>(a, grid, stream);
+  if (s.rows == 16) return launch_mma<64, 1, 1, 4>(a, grid, stream);  // (heads of 48)
+  if (s.rows == 32) return launch_mma<64, 2, 1, 4>(a, grid, stream);
+  return launch_mma<64, 2, 2, 4>(a, grid, stream);
 }

@@ -260,9 +260,9 @@ _prototypes = {
                                           c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                           c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float,
                                           c_int, c_void_p],
-    ("attention_shared", "dllm_attention_shared_shape"): [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int],
+    ("attention_shared", "dllm_attention_shared_shape"): [c_int, c_int, c_int, c_int, c_int, c_int, c_int],
     ("attention_shared", "dllm_attention_shared"): [
-        c_int, c_void_p, c_void_p, c_void_p, c_longlong, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+        c_void_p, c_void_p, c_void_p, c_longlong, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
         c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
     ("beam_reorder", "dllm_beam_reorder"): [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                             c_void_p],
@@ -2395,16 +2395,10 @@ def attention_shared_supported(cache) -> bool:
         and cache.value_dim == cache.head_dim and not cache.keys_only
 
 
-def _shared_kind(cache, kind: int) -> int:
-    # (a TMA coordinate is an int: storage of more rows takes the kernel that addresses by 64 bits)
-    return 1 if kind < 0 and cache.dtype == torch.bfloat16 and cache.storage.shape[0] * 2 * cache.kv_heads * 64 > 0x7fffffff else kind
-
-
-def attention_shared_scratch(cache, heads: int, groups: int, max_rows: int, max_context: int,
-                             kind: int = -1) -> tuple[int, int]:
+def attention_shared_scratch(cache, heads: int, groups: int, max_rows: int, max_context: int) -> tuple[int, int]:
     """(floats of scratch, int32 tickets) that `attention_shared` needs for these bounds."""
     shape = _fn("attention_shared", "dllm_attention_shared_shape")(
-        _shared_kind(cache, kind), _code(cache.dtype), heads, cache.kv_heads, cache.head_dim, groups, max_rows, max_context)
+        _code(cache.dtype), heads, cache.kv_heads, cache.head_dim, groups, max_rows, max_context)
     if shape <= 0:
         raise KernelError(f"attention_shared: {_STATUS.get(shape, shape)} ({heads} heads on {cache.kv_heads}, {groups} groups "
                           f"of {max_rows}, contexts of {max_context})")
@@ -2415,7 +2409,7 @@ def attention_shared_scratch(cache, heads: int, groups: int, max_rows: int, max_
 
 def attention_shared(out: torch.Tensor, q: torch.Tensor, cache, heads: int, scale: float, window: int, slots: torch.Tensor,
                      positions: torch.Tensor, groups: torch.Tensor, shared: torch.Tensor, max_rows: int, max_context: int,
-                     scratch: torch.Tensor, tickets: torch.Tensor, kind: int = -1) -> None:
+                     scratch: torch.Tensor, tickets: torch.Tensor) -> None:
     """Attention of a few new tokens a group, where a group's tokens share pages (csrc/attention_shared.cu): the beams of a
     prompt, or a short chunk appended to a sequence. q, out [tokens, heads * head_dim] in the cache's type (float32 or
     bfloat16; head sizes that are multiples of 8 up to 256).
@@ -2423,8 +2417,7 @@ def attention_shared(out: torch.Tensor, q: torch.Tensor, cache, heads: int, scal
     groups [count + 1], the groups' first tokens (they follow one another); shared [count], how many pages from the first on
     are the same in the table rows of all of a group's tokens (more than there are: all). A group has at most `max_rows` tokens (more:
     `raise_if_failed` says so) and positions lie below `max_context`. scratch, tickets: `attention_shared_scratch`; the
-    tickets are int32 zeros, left zero. kind -1 lets the sizes choose the kernel; 0, 1, 2 name fused multiply-adds, mma.sync
-    (bfloat16, head sizes that are multiples of 16 up to 128) and tcgen05 (of those, 64 and more)."""
+    tickets are int32 zeros, left zero."""
     _cuda(out, q, slots, positions, groups, shared, scratch, tickets)
     count, tokens, width = groups.numel() - 1, q.shape[0], heads * cache.head_dim
     if not attention_shared_supported(cache):
@@ -2439,13 +2432,13 @@ def attention_shared(out: torch.Tensor, q: torch.Tensor, cache, heads: int, scal
     if not (slots.dtype is i32 and positions.dtype is i32 and groups.dtype is i32 and shared.dtype is i32 and tickets.dtype is i32
             and scratch.dtype is torch.float32):
         raise KernelError("attention_shared: scratch is float32, what describes the step int32")
-    floats, words = attention_shared_scratch(cache, heads, max(count, 1), max_rows, max_context, kind)
+    floats, words = attention_shared_scratch(cache, heads, max(count, 1), max_rows, max_context)
     if scratch.numel() < floats or tickets.numel() < words:
         raise KernelError(f"attention_shared: scratch of {scratch.numel()} floats and {tickets.numel()} tickets: {floats} and {words}")
     if max_context > cache.max_pages * cache.page_size:
         raise KernelError(f"attention_shared: contexts of {max_context} in table rows of {cache.max_pages} pages")
     _check(_fn("attention_shared", "dllm_attention_shared")(
-        _shared_kind(cache, kind), out.data_ptr(), q.data_ptr(), cache.base_ptr, cache.storage.shape[0], cache.page_table.data_ptr(), cache.max_pages, cache.page_size,
+        out.data_ptr(), q.data_ptr(), cache.base_ptr, cache.storage.shape[0], cache.page_table.data_ptr(), cache.max_pages, cache.page_size,
         _code(cache.dtype), heads, cache.kv_heads, cache.head_dim, slots.data_ptr(), positions.data_ptr(), groups.data_ptr(),
         shared.data_ptr(), count, max_rows, max_context, float(scale), int(window or 0), scratch.data_ptr(), tickets.data_ptr(),
         _status_word().data_ptr(), _stream()), "attention_shared",
