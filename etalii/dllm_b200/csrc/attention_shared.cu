@@ -308,15 +308,15 @@ __device__ __forceinline__ void finish(Plan& p, const Args& a, const float* x, i
   }
   if (size > 1) cluster_sync();  // nobody leaves while others read its result
   if (clusters == 1) return;
-  __threadfence();
   __syncthreads();
   if (threadIdx.x == 0) {
+    __threadfence();  // (what the block has written, which the barrier has shown to this thread, before the ticket)
     p.last = atomicAdd(&a.tickets[pair], 1u) == (unsigned)(a.splits - 1);
+    __threadfence();
     if (p.last) a.tickets[pair] = 0u;
   }
   __syncthreads();
   if (!p.last) return;
-  __threadfence();
   // the last block: what each cluster's part counts [cluster][row], then the rows' sums
   float2* all_ml = reinterpret_cast<float2*>(weight);
   for (int i = threadIdx.x; i < clusters * ROWS; i += blockDim.x)

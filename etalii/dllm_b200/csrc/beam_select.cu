@@ -13,22 +13,26 @@
 //     beam lives. A sequence that is done keeps its pool, and its places get score -inf.
 //
 // One pass over the logits, in two steps of one launch:
-//   1. A block takes a stretch of a row, at most 16,384 logits that stay in its threads' registers. The threads form
-//      GROUPS groups, at least as many as there are beams; the smallest of the groups' maxima is a bound that at least
-//      `beams` logits reach and few do: of logits in any order all groups' maxima lie within the best GROUPS H(GROUPS),
-//      about 54 of 16 groups and 130 of 32. What reaches it goes to a list, and each entry counts what is before it.
-//      A list that does not hold them all (many equal logits) is given up for `beams` passes over the registers.
-//      The sum of exponentials goes by the block's own maximum.
+//   1. A block walks a stretch of a row in tiles of 256 threads x 4 * REG logits, a thread with a maximum and a sum of its own. The
+//      threads form GROUPS groups, at least as many as there are beams; the smallest of the groups' maxima so far is a bound that
+//      at least `beams` logits reach and few do: of logits in any order all groups' maxima lie within the best
+//      GROUPS H(GROUPS), about 54 of 16 groups and 130 of 32. What of a tile reaches the bound goes to a list, which is thinned out by the
+//      latest bound when it fills; at the end each entry counts what is before it. A list that does not hold them all (many
+//      equal logits) is given up for `beams` passes over the stretch.
 //   2. The block that finishes last for its sequence (a ticket counter; nobody waits) joins the stretches' sums,
 //      makes the totals and chooses among the stretches' lists the same way; a warp deals out places and pool.
-// Bound by HBM where the rows are many, by the latency of the two steps where they are few.
+// Bound by HBM where the rows are many, by the latency of the two steps where they are few. Blocks of a stretch that fits
+// their registers (4,096 of them for 512 rows of 128,256 instead of 512) spent most of their time on what a block costs.
+#include <float.h>
+
 #include "common.cuh"
 
 namespace {
-constexpr int THREADS = 512;
+constexpr int THREADS = 256;
 constexpr int MAX_BEAMS = 32, MAX_STOPS = 8;
-constexpr int LIST = 1024;       // candidates a block orders by counting
-constexpr int MAX_REG = 8;       // float4 a thread holds of its stretch
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int LIST = 1024;       // candidates a block keeps
+constexpr int PLACES = 148 * 4;  // blocks that are resident at a time
 
 struct Args {
   const float* logits;
@@ -56,41 +60,73 @@ __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
 }
 
 struct Shared {
-  float list_x[LIST];
-  int list_t[LIST];
+  // a stretch's candidates as words that order them (`word_of`); a sequence's as logit and token, total, beam
+  unsigned long long list[LIST];
   float list_total[LIST];
   int list_beam[LIST];
-  float group_max[THREADS / 32][MAX_BEAMS];
-  float warp_f[THREADS / 32];
-  int list_n, last;
+  float group_max[2][THREADS / 32][MAX_BEAMS];
+  float warp_m[THREADS / 32], warp_f[THREADS / 32];
+  int list_n, seen_n[2], kept_n, last;
   unsigned long long best[2];
   float lse[MAX_BEAMS], score[MAX_BEAMS];
   Candidate chosen[MAX_BEAMS];
   Candidate stop[MAX_BEAMS * MAX_STOPS];
+  float chosen_total[MAX_BEAMS], stop_total[MAX_BEAMS * MAX_STOPS];
   Candidate ended[MAX_BEAMS];
   int n_ended;
   int stops[MAX_STOPS];
 };
+
+// two floats at a time
+typedef unsigned long long Two;
+__device__ __forceinline__ Two two(float x, float y) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 apart(Two v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 
 __device__ __forceinline__ unsigned ordered(float v) {  // larger floats have larger words; no NaN comes here
   unsigned b = __float_as_uint(v + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// The smallest of the groups' maxima of v, and the block's largest: every thread gets both. A thread belongs to group
-// threadIdx.x % GROUPS, so that a short stretch has something of every group.
+// Orders a row's candidates: by logit, then by the lower token.
+__device__ __forceinline__ unsigned long long word_of(float logit, int token) {
+  return ((unsigned long long)ordered(logit) << 32) | (unsigned)(0x7fffffff - token);
+}
+__device__ __forceinline__ float logit_of(unsigned long long word) {
+  const unsigned w = (unsigned)(word >> 32);
+  return __uint_as_float(w & 0x80000000u ? w & 0x7fffffffu : ~w);
+}
+__device__ __forceinline__ int token_of(unsigned long long word) { return 0x7fffffff - (int)(unsigned)word; }
+
+// The smallest of the groups' maxima of v, which every thread gets. A thread belongs to group threadIdx.x % GROUPS, so that
+// a short stretch has something of every group. `set`: 0 and 1 in turn.
 template <int GROUPS>
-__device__ __forceinline__ float bound_of(float v, Shared& sh, float& largest) {
-  constexpr int WARPS = THREADS / 32;
+__device__ __forceinline__ float bound_of(float v, Shared& sh, int set) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 16; o >= GROUPS; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if (lane < GROUPS) sh.group_max[threadIdx.x >> 5][lane] = v;
+  if (lane < GROUPS) sh.group_max[set][threadIdx.x >> 5][lane] = v;
   __syncthreads();
   float low = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < WARPS; ++w) low = fmaxf(low, sh.group_max[w][lane % GROUPS]);
-  largest = warp_max(low);
+  for (int w = 0; w < THREADS / 32; ++w) low = fmaxf(low, sh.group_max[set][w][lane % GROUPS]);
 #pragma unroll
   for (int o = GROUPS / 2; o > 0; o >>= 1) low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
   return low;
@@ -114,126 +150,168 @@ __device__ __forceinline__ void leave_as_is(const Args& a, int b, int* history) 
 }
 
 template <int REG, int GROUPS>
-__global__ void __launch_bounds__(THREADS, 2) select_kernel(const Args a) {
+__global__ void __launch_bounds__(THREADS, 4) select_kernel(const Args a) {
   __shared__ Shared sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.y, b = row / a.beams_in, k = row % a.beams_in;
   const int part = blockIdx.x, parts = gridDim.x;
   const int beams = a.beams, vocab = a.vocab;
-  if (tid == 0) { sh.list_n = 0; sh.n_ended = 0; }
+  if (tid == 0) sh.list_n = sh.n_ended = sh.seen_n[0] = sh.seen_n[1] = 0;
   pdl_launch_dependents();
   pdl_wait();
-  const int run_step = a.steps ? a.steps[0] : 0, sequences = gridDim.y / a.beams_in;
-  const int step = a.produced[0] + run_step;
+  // ---- the stretch: whole fours where addresses are multiples of 16 bytes; the up to three logits before and behind those are
+  // `extra` of threads 0 to 2 and 4 to 6. The first tile is asked for before anything is looked at.
+  const float* x = a.logits + (size_t)row * a.row_stride;
+  const int lo = min(vocab, part * a.stretch), hi = min(vocab, lo + a.stretch);
+  const int first = min(hi, lo + (int)((0 - (reinterpret_cast<uintptr_t>(x + lo) >> 2)) & 3));
+  const int fours = (hi - first) >> 2, behind = first + 4 * fours;
+  const float4* x4 = reinterpret_cast<const float4*>(x + first);
+  float v[4 * REG];
+  auto load = [&](int tile) {
+#pragma unroll
+    for (int r = 0; r < REG; ++r) {
+      float4 four = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      const int at = (tile * REG + r) * THREADS + tid;
+      if (at < fours) four = __ldcs(x4 + at);
+      v[4 * r] = four.x; v[4 * r + 1] = four.y; v[4 * r + 2] = four.z; v[4 * r + 3] = four.w;
+    }
+  };
+  load(0);
+  int extra_at = -2;
+  if (tid < 3 && lo + tid < first) extra_at = lo + tid;
+  if (tid >= 4 && tid < 7 && behind + tid - 4 < hi) extra_at = behind + tid - 4;
+  const float extra = extra_at >= 0 ? __ldcs(x + extra_at) : -INFINITY;
+  const int run_step = a.steps ? a.steps[0] : 0, step = a.produced[0] + run_step, sequences = gridDim.y / a.beams_in;
+  const bool over = a.done[b] != 0, alive = a.scores[(size_t)b * a.beams_in + k] > -INFINITY;
+  if (tid < a.n_stops) sh.stops[tid] = a.stop_ids[tid];
   // where the parents of this step are kept too
   int* history = a.history && run_step < a.history_steps ? a.history + ((size_t)run_step * sequences + b) * beams : nullptr;
-  if (a.done[b]) {
+  if (over) {
     if (k == 0 && part == 0) leave_as_is(a, b, history);
     return;
   }
-  if (tid < a.n_stops) {
-    int id = a.stop_ids[tid];
-    for (int s = 0; s < tid; ++s) id = a.stop_ids[s] == id ? -1 : id;  // (one named twice counts once)
-    sh.stops[tid] = id;
-  }
+  __syncthreads();
+  const int n_stops = a.n_stops;
+  auto is_stop = [&](int i) {
+    bool stop = false;
+    for (int s = 0; s < n_stops; ++s) stop = stop || sh.stops[s] == i;
+    return stop;
+  };
   float* mine = a.scratch + ((size_t)row * parts + part) * (2 + 2 * beams);
-  if (a.scores[(size_t)b * a.beams_in + k] > -INFINITY) {
-    // ---- the stretch, in registers
-    const float* x = a.logits + (size_t)row * a.row_stride;
-    const int lo = part * a.stretch, hi = min(vocab, lo + a.stretch);
-    // pieces of four begin where addresses are multiples of 16 bytes
-    const int skew = (int)((reinterpret_cast<uintptr_t>(x + lo) >> 2) & 3);
-    float v[4 * REG];
-#pragma unroll
-    for (int r = 0; r < REG; ++r) {
-      int i = lo - skew + 4 * (r * THREADS + tid);
-      if (i >= lo && i + 3 < hi) {
-        float4 four = __ldcs(reinterpret_cast<const float4*>(x + i));
-        v[4 * r] = four.x; v[4 * r + 1] = four.y; v[4 * r + 2] = four.z; v[4 * r + 3] = four.w;
-      } else {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) v[4 * r + u] = i + u >= lo && i + u < hi ? __ldcs(x + i + u) : -INFINITY;
-      }
-    }
-    __syncthreads();  // (the stop tokens are there)
-    const int n_stops = a.n_stops;
-    float top = -INFINITY, keep = -INFINITY;  // of all logits; of those that may be chosen
-#pragma unroll
-    for (int r = 0; r < REG; ++r) {
-      float four = fmaxf(fmaxf(v[4 * r], v[4 * r + 1]), fmaxf(v[4 * r + 2], v[4 * r + 3]));
-      top = fmaxf(top, four);
-    }
-    keep = top;
-    if (n_stops) {  // a thread whose piece holds a stop token looks closer
-      bool holds = false;
-      for (int s = 0; s < n_stops; ++s) {
-        int at = sh.stops[s] - (lo - skew);
-        holds = holds || (sh.stops[s] >= lo && sh.stops[s] < hi && (at >> 2) % THREADS == tid);
-      }
-      if (holds) {
-        keep = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < 4 * REG; ++e) {
-          int i = lo - skew + 4 * ((e >> 2) * THREADS + tid) + (e & 3);
-          bool stop = false;
-          for (int s = 0; s < n_stops; ++s) stop = stop || sh.stops[s] == i;
-          if (!stop) keep = fmaxf(keep, v[e]);
-        }
-      }
-    }
-    float unused, m;
-    {  // the block's maximum over everything, for the sum
-      float t = warp_max(top);
-      if (lane == 0) sh.warp_f[warp] = t;
-    }
-    const float low = bound_of<GROUPS>(keep, sh, unused);
-    m = sh.warp_f[0];
-#pragma unroll
-    for (int w = 1; w < THREADS / 32; ++w) m = fmaxf(m, sh.warp_f[w]);
-    auto is_stop = [&](int i) {
-      bool stop = false;
-      for (int s = 0; s < n_stops; ++s) stop = stop || sh.stops[s] == i;
-      return stop;
+  if (alive) {
+    auto place_of = [&](int tile, int e) { return first + 4 * ((tile * REG + (e >> 2)) * THREADS + tid) + (e & 3); };
+    auto offer = [&](float value, int i) {
+      if (is_stop(i)) return;
+      int at = atomicAdd(&sh.list_n, 1);
+      if (at < LIST) sh.list[at] = word_of(value, i);
     };
-    float sum = 0.f;
-    const float shift = m > -INFINITY ? m : 0.f;  // (a stretch of nothing but -inf adds nothing)
+    float m = extra, sum = extra > -INFINITY ? 1.f : 0.f, keep = -INFINITY, low = -INFINITY;
+    if (extra != extra) sum = extra;  // (a NaN is the row's end)
+    if (extra_at >= 0 && !is_stop(extra_at)) keep = extra;
+    float floor_ = -FLT_MAX;
+    int updates = 0;
+    const int tiles = max(1, (fours + REG * THREADS - 1) / (REG * THREADS));
+    for (int tile = 0; tile < tiles; ++tile) {
+      if (tile > 0) load(tile);
+      float top = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < 4 * REG; ++e) {
-      sum += expf(v[e] - shift);
-      if (v[e] >= low && v[e] > -INFINITY) {
-        int i = lo - skew + 4 * ((e >> 2) * THREADS + tid) + (e & 3);
-        if (!is_stop(i)) {
-          int at = atomicAdd(&sh.list_n, 1);
-          if (at < LIST) { sh.list_x[at] = v[e]; sh.list_t[at] = i; }
+      for (int e = 0; e < 4 * REG; ++e) top = fmaxf(top, v[e]);
+      // The bound goes by what may be chosen: what a thread has in a tile beside a stop token does not take part in it (any
+      // logits of at least `beams` groups make a bound).
+      bool beside = false;
+      for (int s = 0; s < n_stops; ++s) {
+        const int at = ((sh.stops[s] - first) >> 2) - tile * REG * THREADS;
+        beside = beside || (sh.stops[s] >= first && sh.stops[s] < behind && at >= 0 && at < REG * THREADS && at % THREADS == tid);
+      }
+      if (!beside) keep = fmaxf(keep, top);
+      if ((tile & (tile - 1)) == 0) {  // a new bound with the first, the second, the third, the fifth, the ninth tile ..: no barrier between
+        if (tid == 0) sh.seen_n[updates & 1] = sh.list_n;  // (of the tiles before; a late entry of the last one may be missing)
+        low = bound_of<GROUPS>(keep, sh, updates & 1);
+        floor_ = fmaxf(low, -FLT_MAX);  // (-inf is no candidate)
+        if (sh.seen_n[updates & 1] > LIST / 2) {  // thin out the list
+          __syncthreads();
+          const int n = min(sh.list_n, LIST);
+          unsigned long long kept[LIST / THREADS];
+#pragma unroll
+          for (int u = 0; u < LIST / THREADS; ++u) kept[u] = u * THREADS + tid < n ? sh.list[u * THREADS + tid] : 0ull;
+          const bool lost = sh.list_n > LIST;
+          __syncthreads();
+          if (tid == 0) sh.list_n = lost ? LIST + 1 : 0;  // (what is lost stays lost)
+          __syncthreads();
+          if (!lost)
+#pragma unroll
+            for (int u = 0; u < LIST / THREADS; ++u)
+              if (kept[u] >= word_of(floor_, 0x7fffffff)) sh.list[atomicAdd(&sh.list_n, 1)] = kept[u];
+          __syncthreads();
+        }
+        ++updates;
+      }
+      const float m_new = fmaxf(m, top), shift = m_new > -INFINITY ? -m_new : 0.f;
+      Two sums[2] = {two(0.f, 0.f), two(0.f, 0.f)};
+      const Two shift2 = two(shift, shift), log2e2 = two(LOG2E, LOG2E);
+      unsigned hits = 0u;  // which of this thread's logits reach the bound
+#pragma unroll
+      for (int r = 0; r < REG; ++r) {
+        const float* four = v + 4 * r;
+        if (fmaxf(fmaxf(four[0], four[1]), fmaxf(four[2], four[3])) >= floor_) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (four[u] >= floor_) hits |= 1u << (4 * r + u);
+        }
+        // (the difference first: it is exact where the weight is large)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float2 y = apart(mul2(add2(two(four[2 * u], four[2 * u + 1]), shift2), log2e2));
+          sums[u] = add2(sums[u], two(fast_exp2(y.x), fast_exp2(y.y)));
         }
       }
+      const float2 all_four = apart(add2(sums[0], sums[1]));
+      sum = sum * (m > -INFINITY ? fast_exp2((m + shift) * LOG2E) : 1.f) + (all_four.x + all_four.y);
+      m = m_new;
+      while (hits) {
+        const int e = __ffs(hits) - 1;
+        hits &= hits - 1;
+        float value = v[0];
+#pragma unroll
+        for (int j = 1; j < 4 * REG; ++j) value = e == j ? v[j] : value;
+        offer(value, place_of(tile, e));
+      }
     }
-    sum = warp_sum(sum);
-    __syncthreads();  // (everybody has read the maxima; the list is whole)
-    if (lane == 0) sh.warp_f[warp] = sum;
+    if (extra >= fmaxf(low, -FLT_MAX)) offer(extra, extra_at);
+    // ---- the stretch's maximum and sum, its best
+    const float warp_top = warp_max(m);
+    sum = warp_sum(m > -INFINITY ? sum * fast_exp2((m - warp_top) * LOG2E) : sum);  // (0 where there is nothing, or a NaN)
+    if (lane == 0) { sh.warp_m[warp] = warp_top; sh.warp_f[warp] = sum; }
+    __syncthreads();
+    if (tid == 0) {
+      float top = -INFINITY, total = 0.f;
+      for (int w = 0; w < THREADS / 32; ++w) top = fmaxf(top, sh.warp_m[w]);
+      for (int w = 0; w < THREADS / 32; ++w)
+        total += sh.warp_m[w] > -INFINITY ? sh.warp_f[w] * fast_exp2((sh.warp_m[w] - top) * LOG2E) : sh.warp_f[w];
+      mine[0] = top;
+      mine[1] = total;
+    }
     const int n = sh.list_n;
     if (n <= LIST) {
       for (int c = tid; c < n; c += THREADS) {
-        float xc = sh.list_x[c];
-        int tc = sh.list_t[c], place = 0;
-        for (int j = 0; j < n; ++j) {
-          float xj = sh.list_x[j];
-          place += xj > xc ? 1 : 0;
-          if (xj == xc && j != c) place += sh.list_t[j] < tc ? 1 : 0;
-        }
-        if (place < beams) { mine[2 + 2 * place] = xc; mine[3 + 2 * place] = __int_as_float(tc); }
+        const unsigned long long mine_word = sh.list[c];
+        if (logit_of(mine_word) < low) continue;  // (in the list by an earlier bound)
+        int place = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) place += sh.list[j] > mine_word ? 1 : 0;
+        if (place < beams) { mine[2 + 2 * place] = logit_of(mine_word); mine[3 + 2 * place] = __int_as_float(token_of(mine_word)); }
       }
+      // (fewer than `beams` that may be chosen: all of them are in the list, whatever the bound)
       for (int c = n + tid; c < beams; c += THREADS) { mine[2 + 2 * c] = -INFINITY; mine[3 + 2 * c] = 0.f; }
     } else {
       // one after another: the best that comes behind the last one. (A word orders by logit, then by the lower token.)
       unsigned long long last = ~0ull;
       for (int c = 0; c < beams; ++c) {
         unsigned long long best = 0;
-#pragma unroll
-        for (int e = 0; e < 4 * REG; ++e) {
-          int i = lo - skew + 4 * ((e >> 2) * THREADS + tid) + (e & 3);
-          if (v[e] > -INFINITY) {
-            unsigned long long word = ((unsigned long long)ordered(v[e]) << 32) | (unsigned)(0x7fffffff - i);
+        for (int i = lo + tid; i < hi; i += THREADS) {
+          const float value = x[i];
+          if (value > -INFINITY) {
+            const unsigned long long word = word_of(value, i);
             if (word < last && word > best && !is_stop(i)) best = word;
           }
         }
@@ -248,220 +326,255 @@ __global__ void __launch_bounds__(THREADS, 2) select_kernel(const Args a) {
         __syncthreads();
         last = sh.best[c & 1];
         if (tid == 0) {
-          unsigned w = (unsigned)(last >> 32);
-          mine[2 + 2 * c] = last ? __uint_as_float(w & 0x80000000u ? w & 0x7fffffffu : ~w) : -INFINITY;
-          mine[3 + 2 * c] = __int_as_float(last ? 0x7fffffff - (int)(unsigned)last : 0);
+          mine[2 + 2 * c] = last ? logit_of(last) : -INFINITY;
+          mine[3 + 2 * c] = __int_as_float(last ? token_of(last) : 0);
         }
       }
     }
-    __syncthreads();
-    if (tid == 0) {
-      float total = 0.f;
-#pragma unroll
-      for (int w = 0; w < THREADS / 32; ++w) total += sh.warp_f[w];
-      mine[0] = m;
-      mine[1] = total;
-    }
   }
   // ---- who is last?
-  __threadfence();
   __syncthreads();
-  if (tid == 0) sh.last = atomicAdd(&a.tickets[b], 1u) == (unsigned)(a.beams_in * parts - 1);
+  if (tid == 0) {
+    __threadfence();  // (what the block has written, which the barrier has shown to this thread, before the ticket)
+    sh.last = atomicAdd(&a.tickets[b], 1u) == (unsigned)(a.beams_in * parts - 1);
+    __threadfence();
+    sh.list_n = 0;
+  }
   __syncthreads();
   if (!sh.last) return;
-  __threadfence();
-  if (tid == 0) { a.tickets[b] = 0u; sh.list_n = 0; }
+  if (tid == 0) a.tickets[b] = 0u;
+  // Everything that is needed is asked for at once.
   const size_t entry = 2 + 2 * (size_t)beams;
   const float* all = a.scratch + (size_t)b * a.beams_in * parts * entry;
+  const int n_lists = a.beams_in * parts, n_entries = n_lists * beams;
+  // (quotients by products: exact while dividend x divisor < 2^32)
+  const unsigned by_beams = 0xffffffffu / (unsigned)beams + 1u, by_parts = 0xffffffffu / (unsigned)parts + 1u;
+  auto list_of = [&](int c) { return beams == 1 ? c : (int)__umulhi((unsigned)c, by_beams); };
+  auto beam_of = [&](int c) { return parts == 1 ? list_of(c) : (int)__umulhi((unsigned)list_of(c), by_parts); };
+  auto pair_at = [&](int c) {
+    const int list = list_of(c);
+    return __ldcg(reinterpret_cast<const float2*>(all + (size_t)list * entry + 2 + 2 * (c - list * beams)));
+  };
+  constexpr int HELD = 4;  // what a thread looks at first stays with it
+  float2 held[HELD];
+#pragma unroll
+  for (int u = 0; u < HELD; ++u) held[u] = tid + u * THREADS < n_entries ? pair_at(tid + u * THREADS) : make_float2(-INFINITY, 0.f);
+  const bool may_end = step >= a.min_tokens;
+  const int n_stop = may_end ? a.beams_in * n_stops : 0;  // (at most THREADS)
+  int stop_beam = 0, stop_token = -1;
+  float stop_logit = -INFINITY;
+  if (tid < n_stop) {
+    stop_beam = tid / n_stops;
+    const int s = tid - stop_beam * n_stops;
+    stop_token = sh.stops[s];
+    for (int j = 0; j < s; ++j) stop_token = sh.stops[j] == stop_token ? -1 : stop_token;  // (one named twice counts once)
+    if (stop_token >= 0 && stop_token < vocab) stop_logit = a.logits[(size_t)(b * a.beams_in + stop_beam) * a.row_stride + stop_token];
+  }
+  const bool on = warp == 0 && lane < beams;  // the first warp has a lane a beam
+  const size_t at = (size_t)b * beams + lane;
+  const float pool = on ? a.finished[at] : -INFINITY;
+  const int pool_step = on ? a.finished_at[2 * at] : -1, pool_beam = on ? a.finished_at[2 * at + 1] : -1;
+  const float length = powf((float)(step + 1), a.penalty);
   // the rows' sums: a warp a row
   for (int r = warp; r < a.beams_in; r += THREADS / 32) {
-    float score = a.scores[(size_t)b * a.beams_in + r], top = -INFINITY, sum = 0.f;
+    const float score = a.scores[(size_t)b * a.beams_in + r];
+    float2 part_ml = lane < parts ? __ldcg(reinterpret_cast<const float2*>(all + ((size_t)r * parts + lane) * entry)) : make_float2(-INFINITY, 0.f);
+    float m = -INFINITY, sum = 0.f;
     if (score > -INFINITY) {
-      for (int p = lane; p < parts; p += 32) top = fmaxf(top, __ldcg(all + ((size_t)r * parts + p) * entry));
-      top = warp_max(top);
-      for (int p = lane; p < parts; p += 32) {
-        float pm = __ldcg(all + ((size_t)r * parts + p) * entry), ps = __ldcg(all + ((size_t)r * parts + p) * entry + 1);
-        sum += pm > -INFINITY ? ps * expf(pm - top) : ps;  // (ps is 0 there, or a NaN)
+      m = part_ml.x;
+      sum = part_ml.y;
+      for (int p = lane + 32; p < parts; p += 32) {
+        part_ml = __ldcg(reinterpret_cast<const float2*>(all + ((size_t)r * parts + p) * entry));
+        const float m_new = fmaxf(m, part_ml.x), shift = m_new > -INFINITY ? m_new : 0.f;
+        sum = (m > -INFINITY ? sum * expf(m - shift) : sum) + (part_ml.x > -INFINITY ? part_ml.y * expf(part_ml.x - shift) : part_ml.y);
+        m = m_new;
       }
-      sum = warp_sum(sum);
     }
+    const float top = warp_max(m);
+    sum = warp_sum(m > -INFINITY ? sum * expf(m - top) : sum);  // (0 where there is nothing, or a NaN)
     if (lane == 0) {
       sh.lse[r] = top + logf(sum);
       sh.score[r] = score > -INFINITY ? score : -INFINITY;
     }
   }
+  for (int c = tid; c < beams; c += THREADS) {
+    sh.chosen[c] = Candidate{-INFINITY, -INFINITY, 0x7fffffff, 0x7fffffff};
+    sh.chosen_total[c] = -INFINITY;
+  }
   __syncthreads();
-  const int n_entries = a.beams_in * parts * beams, per_row = parts * beams;
-  auto load = [&](int c) {
-    Candidate out;
-    out.beam = c / per_row;
-    out.total = -INFINITY;
-    out.logit = -INFINITY;
-    out.token = 0;
-    if (sh.score[out.beam] > -INFINITY) {
-      const float* at = all + (size_t)(c / beams) * entry + 2 + 2 * (c % beams);
-      float2 pair = __ldcg(reinterpret_cast<const float2*>(at));
-      out.logit = pair.x;
-      out.token = __float_as_int(pair.y);
-      float total = (pair.x - sh.lse[out.beam]) + sh.score[out.beam];
-      if (total > -INFINITY) out.total = total;
-    }
-    return out;
+  // a total, -inf where the row has none (what a row without a score left in scratch is not looked at)
+  auto total_of = [&](float logit, int beam) {
+    const float total = (logit - sh.lse[beam]) + sh.score[beam];
+    return sh.score[beam] > -INFINITY && total > -INFINITY ? total : -INFINITY;
   };
-  float top = -INFINITY, unused;
-  for (int c = tid; c < n_entries; c += THREADS) top = fmaxf(top, load(c).total);
-  const float low = bound_of<GROUPS>(top, sh, unused);
-  for (int c = tid; c < n_entries; c += THREADS) {
-    Candidate one = load(c);
-    if (one.total >= low && one.total > -INFINITY) {
-      int at = atomicAdd(&sh.list_n, 1);
-      if (at < LIST) {
-        sh.list_x[at] = one.logit;
-        sh.list_t[at] = one.token;
-        sh.list_total[at] = one.total;
-        sh.list_beam[at] = one.beam;
-      }
-    }
+  auto candidate_at = [&](int c) {
+    const float2 pair = pair_at(c);
+    const int beam = beam_of(c);
+    return Candidate{total_of(pair.x, beam), pair.x, beam, __float_as_int(pair.y)};
+  };
+  float top = -INFINITY, totals[HELD];
+#pragma unroll
+  for (int u = 0; u < HELD; ++u) {
+    const int c = tid + u * THREADS;
+    totals[u] = c < n_entries ? total_of(held[u].x, beam_of(c)) : -INFINITY;
+    top = fmaxf(top, totals[u]);
   }
-  // the totals of the stop tokens, where they may end a text
-  const bool may_end = step >= a.min_tokens;
-  const int n_stop = may_end ? a.beams_in * a.n_stops : 0;
-  for (int c = tid; c < n_stop; c += THREADS) {
-    Candidate one{-INFINITY, -INFINITY, c / a.n_stops, sh.stops[c % a.n_stops]};
-    if (sh.score[one.beam] > -INFINITY && one.token >= 0 && one.token < vocab) {
-      one.logit = a.logits[(size_t)(b * a.beams_in + one.beam) * a.row_stride + one.token];
-      float total = (one.logit - sh.lse[one.beam]) + sh.score[one.beam];
-      if (total > -INFINITY) one.total = total;
-    }
-    sh.stop[c] = one;
+  for (int c = tid + HELD * THREADS; c < n_entries; c += THREADS) top = fmaxf(top, candidate_at(c).total);
+  if (tid < n_stop) {
+    const float total = stop_token >= 0 && stop_token < vocab ? total_of(stop_logit, stop_beam) : -INFINITY;
+    sh.stop[tid] = Candidate{total, stop_logit, stop_beam, stop_token};
+    sh.stop_total[tid] = total;
   }
-  for (int c = tid; c < beams; c += THREADS) sh.chosen[c] = Candidate{-INFINITY, -INFINITY, 0x7fffffff, 0x7fffffff};
+  const float low = bound_of<GROUPS>(top, sh, 0), floor_ = fmaxf(low, -FLT_MAX);
+  auto offer = [&](const Candidate& one) {
+    const int to = atomicAdd(&sh.list_n, 1);
+    if (to < LIST) {
+      sh.list[to] = ((unsigned long long)__float_as_uint(one.logit) << 32) | (unsigned)one.token;
+      sh.list_total[to] = one.total;
+      sh.list_beam[to] = one.beam;
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < HELD; ++u)
+    if (totals[u] >= floor_) offer(Candidate{totals[u], held[u].x, beam_of(tid + u * THREADS), __float_as_int(held[u].y)});
+  for (int c = tid + HELD * THREADS; c < n_entries; c += THREADS) {
+    const Candidate one = candidate_at(c);
+    if (one.total >= floor_) offer(one);
+  }
   __syncthreads();
+  auto listed = [&](int c) {
+    return Candidate{sh.list_total[c], __uint_as_float((unsigned)(sh.list[c] >> 32)), sh.list_beam[c], (int)(unsigned)sh.list[c]};
+  };
   const int n = sh.list_n;
   if (n <= LIST) {
     for (int c = tid; c < n; c += THREADS) {
-      Candidate one{sh.list_total[c], sh.list_x[c], sh.list_beam[c], sh.list_t[c]};
-      int place = 0;
+      const float total = sh.list_total[c];
+      int place = 0, equal = 0;
+#pragma unroll 8
       for (int j = 0; j < n; ++j) {
-        float total = sh.list_total[j];
-        place += total > one.total ? 1 : 0;
-        if (total == one.total && j != c) place += before(Candidate{total, sh.list_x[j], sh.list_beam[j], sh.list_t[j]}, one) ? 1 : 0;
+        place += sh.list_total[j] > total ? 1 : 0;
+        equal += sh.list_total[j] == total ? 1 : 0;
       }
-      if (place < beams) sh.chosen[place] = one;
+      const Candidate one = listed(c);
+      if (equal > 1)
+        for (int j = 0; j < n; ++j) place += sh.list_total[j] == total && before(listed(j), one) ? 1 : 0;
+      if (place < beams) {
+        sh.chosen[place] = one;
+        sh.chosen_total[place] = total;
+      }
     }
   } else {
-    // one after another, in the order of (total, beam, logit, token): a round finds the best total behind the last one, and
-    // what shares it goes by a second word
+    // one after another, in the order of (total, beam, logit, token)
     Candidate last{INFINITY, INFINITY, -1, -1};
     for (int c = 0; c < beams; ++c) {
       Candidate best{-INFINITY, -INFINITY, 0x7fffffff, 0x7fffffff};
       for (int e = tid; e < n_entries; e += THREADS) {
-        Candidate one = load(e);
+        const Candidate one = candidate_at(e);
         if (one.total > -INFINITY && (c == 0 || before(last, one)) && before(one, best)) best = one;
       }
-      sh.list_total[tid] = best.total;
-      sh.list_x[tid] = best.logit;
-      sh.list_beam[tid] = best.beam;
-      sh.list_t[tid] = best.token;
+      auto put = [&](const Candidate& one) {
+        sh.list[tid] = ((unsigned long long)__float_as_uint(one.logit) << 32) | (unsigned)one.token;
+        sh.list_total[tid] = one.total;
+        sh.list_beam[tid] = one.beam;
+      };
+      put(best);
       __syncthreads();
       for (int o = THREADS / 2; o > 0; o >>= 1) {
-        if (tid < o) {
-          Candidate one{sh.list_total[tid], sh.list_x[tid], sh.list_beam[tid], sh.list_t[tid]};
-          Candidate other{sh.list_total[tid + o], sh.list_x[tid + o], sh.list_beam[tid + o], sh.list_t[tid + o]};
-          if (before(other, one)) {
-            sh.list_total[tid] = other.total;
-            sh.list_x[tid] = other.logit;
-            sh.list_beam[tid] = other.beam;
-            sh.list_t[tid] = other.token;
-          }
-        }
+        if (tid < o && before(listed(tid + o), listed(tid))) put(listed(tid + o));
         __syncthreads();
       }
-      last = Candidate{sh.list_total[0], sh.list_x[0], sh.list_beam[0], sh.list_t[0]};
-      if (tid == 0) sh.chosen[c] = last;
+      last = listed(0);
+      if (tid == 0) {
+        sh.chosen[c] = last;
+        sh.chosen_total[c] = last.total;
+      }
       __syncthreads();
     }
   }
   __syncthreads();
   // ---- texts that end: stop tokens among the first `beams` of all candidates, in order
-  const float length = powf((float)(step + 1), a.penalty);
-  for (int c = tid; c < n_stop; c += THREADS) {
-    Candidate one = sh.stop[c];
-    if (!(one.total > -INFINITY)) continue;
-    int stops_before = 0, live_before = 0;
-    for (int j = 0; j < n_stop; ++j) stops_before += before(sh.stop[j], one) ? 1 : 0;
-    for (int j = 0; j < beams; ++j) live_before += sh.chosen[j].total > -INFINITY && before(sh.chosen[j], one) ? 1 : 0;
-    if (stops_before + live_before < beams) {
-      sh.ended[stops_before] = Candidate{one.total / length, one.logit, one.beam, one.token};
-      atomicAdd(&sh.n_ended, 1);
+  if (tid < n_stop) {
+    const float total = sh.stop_total[tid];
+    if (total > -INFINITY && total >= sh.chosen_total[beams - 1]) {
+      int stops_before = 0, live_before = 0, equal = 0;
+#pragma unroll 8
+      for (int j = 0; j < n_stop; ++j) {
+        stops_before += sh.stop_total[j] > total ? 1 : 0;
+        equal += sh.stop_total[j] == total ? 1 : 0;
+      }
+#pragma unroll 8
+      for (int j = 0; j < beams; ++j) {
+        live_before += sh.chosen_total[j] > total ? 1 : 0;
+        equal += sh.chosen_total[j] == total ? 1 : 0;
+      }
+      const Candidate one = sh.stop[tid];
+      if (equal > 1) {
+        for (int j = 0; j < n_stop; ++j) stops_before += sh.stop_total[j] == total && before(sh.stop[j], one) ? 1 : 0;
+        for (int j = 0; j < beams; ++j) live_before += sh.chosen_total[j] == total && before(sh.chosen[j], one) ? 1 : 0;
+      }
+      if (stops_before + live_before < beams) {
+        sh.ended[stops_before] = Candidate{total / length, one.logit, one.beam, one.token};
+        atomicAdd(&sh.n_ended, 1);
+      }
     }
   }
   __syncthreads();
   if (warp) return;
   // ---- places and pool: a lane a beam
-  const size_t at = (size_t)b * beams + lane;
-  const bool on = lane < beams;
-  Candidate one = on ? sh.chosen[lane] : Candidate{-INFINITY, -INFINITY, 0x7fffffff, 0};
+  const Candidate one = on ? sh.chosen[lane] : Candidate{-INFINITY, -INFINITY, 0x7fffffff, 0};
   const bool live = on && one.total > -INFINITY;
-  unsigned same = __match_any_sync(0xffffffffu, live ? one.beam : -1 - lane);
+  const unsigned same = __match_any_sync(0xffffffffu, live ? one.beam : -1 - lane);
   const bool stays = live && one.beam < beams && (same & ((1u << lane) - 1u)) == 0u;
-  unsigned taken = __reduce_or_sync(0xffffffffu, stays ? 1u << one.beam : 0u);
-  unsigned others = __ballot_sync(0xffffffffu, on && !stays);
+  const unsigned taken = __reduce_or_sync(0xffffffffu, stays ? 1u << one.beam : 0u);
+  const unsigned others = __ballot_sync(0xffffffffu, on && !stays);
   int place = one.beam;
   if (on && !stays) {
-    int rank = __popc(others & ((1u << lane) - 1u));
-    place = 0;
-    for (int i = 0; i < beams; ++i) {
-      if (taken >> i & 1u) continue;
-      if (rank-- == 0) { place = i; break; }
-    }
+    unsigned free_places = ~taken;
+    for (int rank = __popc(others & ((1u << lane) - 1u)); rank > 0; --rank) free_places &= free_places - 1u;
+    place = __ffs(free_places) - 1;
   }
   if (on) {
-    size_t to = (size_t)b * beams + place;
-    int parent = live ? one.beam : min(place, a.beams_in - 1);
+    const size_t to = (size_t)b * beams + place;
+    const int parent = live ? one.beam : min(place, a.beams_in - 1);
     a.scores_out[to] = live ? one.total : -INFINITY;
     a.parents[to] = parent;
     a.tokens[to] = live ? one.token : 0;
     if (history) history[place] = parent;
   }
   const int n_ended = sh.n_ended;
-  float pool = on ? a.finished[at] : -INFINITY;
-  int pool_step = on ? a.finished_at[2 * at] : -1, pool_beam = on ? a.finished_at[2 * at + 1] : -1;
   int pool_place = lane, ended_place = lane;
-  float ended = lane < n_ended ? sh.ended[lane].total : -INFINITY;
-  for (int j = 0; j < n_ended; ++j) pool_place += sh.ended[j].total > pool ? 1 : 0;
-  for (int j = 0; j < beams; ++j) ended_place += __shfl_sync(0xffffffffu, pool, j) >= ended ? 1 : 0;
+  const float ended = lane < n_ended ? sh.ended[lane].total : -INFINITY;
+  if (n_ended) {
+    for (int j = 0; j < n_ended; ++j) pool_place += sh.ended[j].total > pool ? 1 : 0;
+    for (int j = 0; j < beams; ++j) ended_place += __shfl_sync(0xffffffffu, pool, j) >= ended ? 1 : 0;
+  }
   __syncwarp();
   float worst = -INFINITY;
   if (on && pool_place < beams) {
-    size_t to = (size_t)b * beams + pool_place;
+    const size_t to = (size_t)b * beams + pool_place;
     a.finished_out[to] = pool;
     a.finished_at_out[2 * to] = pool_step;
     a.finished_at_out[2 * to + 1] = pool_beam;
     if (pool_place == beams - 1) worst = pool;
   }
   if (lane < n_ended && ended_place < beams) {
-    size_t to = (size_t)b * beams + ended_place;
+    const size_t to = (size_t)b * beams + ended_place;
     a.finished_out[to] = ended;
     a.finished_at_out[2 * to] = step;
     a.finished_at_out[2 * to + 1] = sh.ended[lane].beam;
     if (ended_place == beams - 1) worst = ended;
   }
   worst = warp_max(worst);
-  float best = warp_max(live ? one.total : -INFINITY);
+  const float best = warp_max(live ? one.total : -INFINITY);
   if (lane == 0)
     a.done_out[b] = (worst > -INFINITY && (a.early || worst >= best / length)) || best == -INFINITY ? 1 : 0;
 }
 
-// Logits a thread holds (in fours): enough blocks to fill the device where the rows are few, long stretches where they are
-// many.
-int registers_for(int rows, int vocab) {
-  for (int reg = MAX_REG; reg > 1; reg >>= 1)
-    if ((long long)rows * ((vocab + THREADS * 4 * reg - 1) / (THREADS * 4 * reg)) >= 2 * 148) return reg;
-  return 1;
+// Stretches a row is cut into: as many as fill the device, of 2,048 logits at least.
+int parts_for(int rows, int vocab) {
+  const int most = (vocab - 1) / 2048 + 1, wanted = PLACES / (rows < PLACES ? rows : PLACES);
+  return wanted < most ? wanted : most;
 }
-// (four logits fewer than fit: a stretch may begin inside a piece of four)
-int parts_for(int vocab, int reg) { return (vocab - 1) / (THREADS * 4 * reg - 4) + 1; }
 
 template <int REG>
 int launch(const Args& a, int sequences, int parts, cudaStream_t stream) {
@@ -474,7 +587,7 @@ int launch(const Args& a, int sequences, int parts, cudaStream_t stream) {
 // Stretches that each of `rows` rows of `vocab` logits is cut into: scratch holds rows x stretches x (2 + 2 beams) floats.
 DLLM_EXPORT int dllm_beam_select_parts(int rows, int vocab) {
   if (rows <= 0 || vocab <= 0) return DLLM_BAD_ARGUMENT;
-  return parts_for(vocab, registers_for(rows, vocab));
+  return parts_for(rows, vocab);
 }
 
 // See the head of the file. `logits` [sequences * beams_in, vocab] with a row stride; `scores` [sequences, beams_in]; finished,
@@ -492,15 +605,10 @@ DLLM_EXPORT int dllm_beam_select(const float* logits, long long row_stride, cons
     return DLLM_BAD_ARGUMENT;
   if (beams_in > MAX_BEAMS || beams > MAX_BEAMS || n_stops > MAX_STOPS || (long long)sequences * beams_in > 65535)
     return DLLM_UNSUPPORTED_SIZE;
-  const int rows = sequences * beams_in, reg = registers_for(rows, vocab), parts = parts_for(vocab, reg);
+  const int rows = sequences * beams_in, parts = parts_for(rows, vocab);
   Args a{logits, row_stride, scores, finished, finished_at, done, produced, steps, stop_ids, scores_out, finished_out,
          finished_at_out, done_out, parents, tokens, history, scratch, tickets, beams_in, beams, vocab, n_stops, min_tokens,
          early, 0, history_steps, penalty};
-  a.stretch = ((vocab - 1) / parts + 4) / 4 * 4;  // stretches of one length, whole fours: at most THREADS * 4 * reg - 4
-  switch (reg) {
-    case 1: return launch<1>(a, sequences, parts, stream);
-    case 2: return launch<2>(a, sequences, parts, stream);
-    case 4: return launch<4>(a, sequences, parts, stream);
-    default: return launch<8>(a, sequences, parts, stream);
-  }
+  a.stretch = ((vocab - 1) / parts + 4) / 4 * 4;  // stretches of one length, whole fours
+  return a.stretch <= THREADS * 8 ? launch<2>(a, sequences, parts, stream) : launch<8>(a, sequences, parts, stream);
 }
