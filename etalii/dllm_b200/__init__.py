@@ -12,4 +12,8 @@ def __getattr__(name):
         from .engine.engine import Engine
 
         return Engine
+    if name == "BeamOptions":
+        from .sampling.beams import BeamOptions
+
+        return BeamOptions
     raise AttributeError(name)

@@ -125,6 +125,7 @@ class PagedCache:
         self.needs = list(needs)
         self._groups: list[_KvGroup] = []
         self._state: dict[int, torch.Tensor | None] = {}
+        self._beam_rows = None
         self._where: dict[int, tuple[_KvGroup, int]] = {}
         by_need: dict[CacheNeed, list[int]] = {}
         for entry, need in enumerate(self.needs):
@@ -211,6 +212,43 @@ class PagedCache:
                 have.append(page)
                 group.table_host[slot, index] = page
                 group.dirty.add(slot)
+
+    def fork(self, source: int, slots: Sequence[int], new_tokens: int) -> None:
+        """Lets the new sequences in `slots` (taken, still empty) go on from where `source` is, all of them `new_tokens` further:
+        they share its full pages, which `source` goes on holding (it must outlive them), and have pages of their own from
+        the one it is filling on. What that page and the states hold is taken over on the device (`ops.beam_reorder`). The pages
+        of all of them are taken at once: from then on the page tables are the device's (a row that is not reserved again
+        is not copied again)."""
+        length = self.lengths[source]
+        if not self.slots.is_held(source):
+            raise CacheError(f"slot {source} is not in use")
+        for slot in slots:
+            if not self.slots.is_held(slot) or self.lengths[slot] or any(group.pages_of[slot] for group in self._groups):
+                raise CacheError(f"slot {slot} is not a new sequence's")
+        self.reserve(source, new_tokens)
+        full = length // self.page_size
+        end = -(-(length + new_tokens) // self.page_size)
+        for group in self._groups:
+            if group.pool.free < len(slots) * (end - full):
+                raise CacheError(f"out of pages: {len(slots) * (end - full)} wanted, {group.pool.free} of {group.pool.count} free")
+        for slot in slots:
+            self.lengths[slot] = length
+            for group in self._groups:
+                own = group.pool.take(end - full)
+                group.pages_of[slot] = [None] * full + own
+                group.table_host[slot, :full] = group.table_host[source, :full]
+                group.table_host[slot, full:end] = own
+                group.dirty.add(slot)
+
+    def beam_rows(self):
+        """What a sequence keeps, as the list that `ops.beam_reorder` moves (made once: storage stays where it is)."""
+        if self._beam_rows is None:
+            from .beams import CacheRows
+
+            pages = [(g.storage, g.table, g.need.kv_heads, g.need.head_dim,
+                      0 if g.need.keys_only else g.need.value_dim or g.need.head_dim) for g in self._groups]
+            self._beam_rows = CacheRows(pages, [s for s in self._state.values() if s is not None], self.page_size)
+        return self._beam_rows
 
     def advance(self, slot: int, new_tokens: int) -> None:
         self.lengths[slot] += new_tokens

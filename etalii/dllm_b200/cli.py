@@ -4,6 +4,7 @@ standard output and `fingerprint: ... tokens: ... finish: ...` on standard error
 library takes and returns ids; text is the tokenizer's business).
 
     dllm-b200 --model DIR [--dtype bfloat16|float32] [--device cuda:0] generate --prompt-ids 1,2,3 --max-tokens 64
+    dllm-b200 --model DIR generate --prompt-ids 1,2,3 --max-tokens 64 --beams 4 [--length-penalty 1.0] [--early-stopping]
     dllm-b200 --model DIR info
     dllm-b200 --model DIR [--dtype ...] replay --out DIR --max-tokens N < steps.jsonl
     dllm-b200 --model DIR [--dtype ...] bench [--batch 8] [--prompt-tokens 512] [--new-tokens 64] [--repeats 5]
@@ -47,6 +48,12 @@ def build_parser() -> argparse.ArgumentParser:
     generate.add_argument("--ignore-eos", action="store_true", help="write past the model's end-of-sequence")
     generate.add_argument("--stop-token-id", type=int, action="append", default=[],
                           help="also end at this token id (repeatable)")
+    generate.add_argument("--beams", type=int, default=0,
+                          help="beam search with this many beams: prints each prompt's best texts, best first")
+    generate.add_argument("--length-penalty", type=float, default=1.0,
+                          help="beam search: a text's score is its log probability over (tokens) ** LENGTH_PENALTY")
+    generate.add_argument("--early-stopping", action="store_true",
+                          help="beam search: end as soon as as many texts have ended as there are beams")
 
     commands.add_parser("info", help="the model's configuration and size")
 
@@ -134,6 +141,18 @@ def main(argv: list[str] | None = None) -> int:
     except ValueError as error:
         print(f"error: {error}", file=sys.stderr)
         return 2
+    search = None
+    if args.beams:
+        from .sampling.beams import BeamOptions
+
+        if args.n > 1 or args.temperature > 0:
+            print("error: --beams does not go with --n or --temperature", file=sys.stderr)
+            return 2
+        try:
+            search = BeamOptions(beams=args.beams, length_penalty=args.length_penalty, early_stopping=args.early_stopping)
+        except ValueError as error:
+            print(f"error: {error}", file=sys.stderr)
+            return 2
     from .engine.engine import Engine
 
     try:
@@ -141,6 +160,21 @@ def main(argv: list[str] | None = None) -> int:
     except (ValueError, OSError, RuntimeError) as error:  # weights that do not fit, no CUDA device, a failed build
         print(f"error: {error}", file=sys.stderr)
         return 2
+    if search is not None:
+        try:
+            found = engine.beam_search(prompts, args.max_tokens, search, ignore_eos=args.ignore_eos,
+                                       stop_token_ids=args.stop_token_id, min_tokens=args.min_tokens)
+        except (ValueError, RuntimeError) as error:
+            print(f"error: {error}", file=sys.stderr)
+            return 2
+        for index, texts in enumerate(found):
+            if len(prompts) > 1:
+                print(f"--- prompt {index}", file=sys.stderr)
+            for text in texts:
+                print(" ".join(str(t) for t in text.tokens))
+                print(f"score: {text.score:.6f}  fingerprint: {text.fingerprint}  tokens: {len(text.tokens)}  "
+                      f"finish: {text.finish_reason}", file=sys.stderr)
+        return 0
     try:
         # every prompt's N choices, all prompts together, in ONE call: the engine cuts the list into as many batches
         # as the cache needs; choice c of every prompt draws from the stream of seed + c

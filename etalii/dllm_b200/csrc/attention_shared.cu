@@ -804,7 +804,7 @@ __global__ void __launch_bounds__(Shape<BOXES, ROWS>::THREADS, 1)
   pdl_launch_dependents();
   pdl_wait();
   if (warp >= 1 && warp < SOFT_WARPS) {  // (beside the first warp, which makes the plan)
-    // the queries: rows beyond the tile and dimensions beyond the head are zeros; they carry the scale's sign
+    // the queries: rows beyond the tile and dimensions beyond the head are zeros; they carry the scale's sign, or that it is 0
     const int first = a.cuts[blockIdx.z / a.tiles], row0 = (int)(blockIdx.z % a.tiles) * ROWS;
     const int rows = (a.cuts[blockIdx.z / a.tiles + 1] - first) * per_kv - row0;
     const bf16* q = static_cast<const bf16*>(a.q);
@@ -813,6 +813,7 @@ __global__ void __launch_bounds__(Shape<BOXES, ROWS>::THREADS, 1)
       uint4 v = make_uint4(0u, 0u, 0u, 0u);
       if (r < rows && c * 8 < hd)
         v = *reinterpret_cast<const uint4*>(q + ((size_t)(first + row / per_kv) * a.heads + kv * per_kv + row % per_kv) * hd + c * 8);
+      if (a.scale == 0.f) v = make_uint4(0u, 0u, 0u, 0u);
       if (a.scale < 0.f) { v.x ^= 0x80008000u; v.y ^= 0x80008000u; v.z ^= 0x80008000u; v.w ^= 0x80008000u; }
       *reinterpret_cast<uint4*>(q_s + (c >> 3) * (ROWS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
     }
@@ -919,7 +920,8 @@ __global__ void __launch_bounds__(Shape<BOXES, ROWS>::THREADS, 1)
       const bool real = row < p.rows;
       const int token = real ? (p.row0 + row) / per_kv - p.row0 / per_kv : 0;
       const int high = real ? p.position[token] : -1, low = real ? p.low[token] : 0;
-      const float scale = fabsf(a.scale) * 1.4426950408889634f;  // (the queries carry its sign: the largest product is the largest score)
+      // (the queries carry the sign: the largest product is the largest score; and a masked product is -inf, which 0 must not meet)
+      const float scale = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
       const Two scale2 = two(scale, scale);
       float m_run = -INFINITY;  // of this lane's row
       Two l[16];                // of all 32 rows, this thread's keys
@@ -977,7 +979,7 @@ __global__ void __launch_bounds__(Shape<BOXES, ROWS>::THREADS, 1)
         }
         asm volatile("bar.sync %0, 128;" ::"r"(2 + g * S::HALVES + half) : "memory");
         const float largest = fmaxf(fmaxf(maxima[lane], maxima[ROWS + lane]), fmaxf(maxima[2 * ROWS + lane], maxima[3 * ROWS + lane]));
-        const float top = largest > -INFINITY ? largest * scale : -INFINITY;  // (a scale of 0 makes no NaN of it)
+        const float top = largest * scale;
         float fade = 1.f;
         if (top > m_run) {
           if (m_run > -INFINITY) fade = fast_exp2(m_run - top);  // (else the row's outputs are zeros so far)

@@ -20,7 +20,9 @@ from ..sampling.options import SamplingOptions
 from ..sampling.sampler import Sampler
 from ..weights.loader import load_weights
 from ..weights.random_init import random_tensors
+from ..sampling.beams import BeamOptions
 from .batch import BatchBuffers
+from .beam import BeamGraph, BeamResult, SharedRows, plan_beam_batches, search_batch
 from .decode import DecodeGraph
 from .generate import BatchRun, GenerationResult, check_prompts, plan_batches, run_batches
 from .model import Model
@@ -53,14 +55,16 @@ def _token_array(tokens) -> np.ndarray:
 class Engine:
     def __init__(self, config, tensors, dtype="bfloat16", device="cuda:0", max_tokens: int | None = None,
                  max_length: int | None = None, max_slots: int | None = None, cuda_graphs: bool = True,
-                 decode_chunk: int = 16, decode_logits: bool = False) -> None:
+                 decode_chunk: int = 16, decode_logits: bool = False, split_chunks: int = 0) -> None:
         """`max_length`: the longest sequence the cache holds (default: the model's max_position_embeddings).
         `max_tokens`: the most tokens all live sequences hold together, each rounded up to whole pages of 64
         (default: four sequences of max_length). `cuda_graphs`: replay decode steps as CUDA graphs; switched
         off by itself when a part or block of the model declares `CAPTURABLE = False` (a part made of allocating
         torch ops: a captured graph cannot hold those). `decode_chunk`: decode steps between looks at the chosen tokens.
         `decode_logits`: decode runs always compute the logits (they stay readable in the run's buffer); by default
-        a greedy run lets the head product choose the token itself and stores no logits."""
+        a greedy run lets the head product choose the token itself and stores no logits. `split_chunks`: steps in which
+        sequences bring at most this many new tokens (and one of them more than one) cut their contexts' keys over the
+        device (`ops.attention_shared`), where the parts can: for a few tokens appended to long contexts. 0: never."""
         if not torch.cuda.is_available():
             raise RuntimeError("no CUDA device: this library has no CPU path")
         self.config = config
@@ -81,6 +85,7 @@ class Engine:
         self.cuda_graphs = bool(cuda_graphs) and self.model.capturable()
         self.decode_chunk = int(decode_chunk)
         self.decode_logits = bool(decode_logits)
+        self.split_chunks = int(split_chunks)
         self._graphs: dict = {}
         self.stats: dict = {}
 
@@ -139,12 +144,20 @@ class Engine:
             starts.append(self.cache.length(slot))
         self.cache.sync_tables()
         batch = self.buffers.fill(slots, new_tokens, starts, want)
+        if 1 < batch.max_new <= self.split_chunks:
+            batch.shared = self._shared_rows(batch)
         logits = self.model.forward(batch)
         for slot, tokens in zip(slots, new_tokens):
             self.cache.advance(slot, len(tokens))
         self.steps_run += 1
         self.last_batch = batch
         return logits
+
+    def _shared_rows(self, batch) -> SharedRows:
+        """Every sequence's new tokens as a group of `ops.attention_shared`: all pages in common."""
+        packed = [slot for slot, count in zip(batch.h_slots, batch.h_new) for _ in range(count)]
+        both = torch.tensor(packed + [self.cache.max_pages] * batch.n_seqs, dtype=torch.int32, device=self.rt.device)
+        return SharedRows(both[:len(packed)], batch.cu_seqlens, both[len(packed):], batch.max_new)
 
     def check(self) -> None:
         """Raises `KernelError` if a kernel of a step that has finished reported that its results are invalid."""
@@ -274,6 +287,44 @@ class Engine:
 
         return run_batches(prompts, batches, make_run, start, prefill, decode, finish, chunk=self.decode_chunk,
                            free_chunk=DecodeGraph.CAPACITY)
+
+    def beam_search(self, prompts: Sequence[Sequence[int]], max_new_tokens: int = 64, options: BeamOptions | None = None,
+                    stop_token_ids: Sequence[int] | None = None, ignore_eos: bool = False, max_batch: int | None = None,
+                    min_tokens: int = 0) -> list[list[BeamResult]]:
+        """The options.beams best continuations of every prompt (lists of token ids), best first, as many batches one after
+        another as the cache needs. Stop ids as for `generate` (at most eight); a text cannot end before it has `min_tokens`
+        tokens. Beams hold pages of their own behind the prompt: see `max_tokens`."""
+        options = options or BeamOptions()
+        if min_tokens < 0:
+            raise ValueError("min_tokens must be non-negative")
+        prompts = [np.asarray(p, dtype=np.int64).reshape(-1) for p in prompts]
+        window = min(self.context_length, self.max_length)
+        check_prompts(prompts, self.vocab_size, window)
+        stops = set() if ignore_eos else set(self.spec.stop_token_ids)
+        stops.update(int(t) for t in (stop_token_ids or ()))
+        if len(stops) > ops.MAX_BEAM_STOPS:
+            raise ValueError(f"{len(stops)} stop tokens: a beam search takes at most {ops.MAX_BEAM_STOPS}")
+        if max_new_tokens <= 0:
+            return [[BeamResult((), 0.0, len(p), "length")] for p in prompts]
+        limits = [min(int(max_new_tokens), window - len(p)) for p in prompts]
+        batches = plan_beam_batches([len(p) for p in prompts], limits, options.beams, self.cache.page_size,
+                                    self.cache.smallest_pool(), self.cache.n_slots, max_batch)
+        out: list[list[BeamResult] | None] = [None] * len(prompts)
+        for indices in batches:
+            found = search_batch(self, [prompts[i] for i in indices], [limits[i] for i in indices], options, frozenset(stops),
+                                 int(min_tokens))
+            for index, results in zip(indices, found):
+                out[index] = results
+        return out  # type: ignore[return-value]
+
+    def _beam_graph(self, sequences: int, options: BeamOptions, longest: int, min_tokens: int, stops: tuple) -> BeamGraph:
+        bound = min(self.max_length, -(-int(longest) // self.CONTEXT_BUCKET) * self.CONTEXT_BUCKET)
+        key = ("beams", sequences, bound, options, min_tokens, stops)
+        graph = self._graphs.get(key)
+        if graph is None:
+            graph = self._graphs[key] = BeamGraph(self, sequences, options, use_graph=self.cuda_graphs, max_context=bound,
+                                                  min_tokens=min_tokens, stops=stops)
+        return graph
 
     def complete(self, prompt: Sequence[int], max_tokens: int = 64,
                  options: SamplingOptions | None = None, **kwargs) -> GenerationResult:

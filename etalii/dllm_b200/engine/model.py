@@ -168,7 +168,7 @@ class Model:
             x = self.embedding.forward(batch.tokens, batch.n_tokens, rt, positions=batch.tok_pos)
         else:
             x = self.embedding.forward(batch.tokens, batch.n_tokens, rt)
-        if self.native_layers is not None and self.native_layers.takes(batch):
+        if self.native_layers is not None and getattr(batch, "shared", None) is None and self.native_layers.takes(batch):
             self.native_layers.run(x, batch, rt)  # every layer's launches from one C++ call
         else:
             embedded = None

@@ -156,7 +156,16 @@ class Attention:
                    out_scale=self.output_scale, out_at=at)
             return
         attended = rt.ws.buffer("attended", (n, q_size), rt.dtype)
-        if batch.is_decode and rt.dtype == torch.bfloat16 and ops.attention_decode_cluster_supported(cache):
+        shared = getattr(batch, "shared", None)
+        if shared is not None and ops.attention_shared_supported(cache):
+            # beams, or a few tokens appended to each sequence: pages in common are read once
+            longest = min(batch.max_context, cache.max_pages * cache.page_size)
+            floats, tickets = ops.attention_shared_scratch(cache, self.num_heads, shared.groups.numel() - 1, shared.max_rows, longest)
+            ops.attention_shared(attended, q, cache, self.num_heads, self.scale, self.window or 0, shared.slots, batch.tok_pos,
+                                 shared.groups, shared.shared, shared.max_rows, longest,
+                                 rt.ws.buffer("shared_scratch", (max(floats, 1),), torch.float32),
+                                 rt.ws.zeros("shared_tickets", tickets, torch.int32))
+        elif batch.is_decode and rt.dtype == torch.bfloat16 and ops.attention_decode_cluster_supported(cache):
             ops.attention_decode_cluster(attended, q, cache, self.num_heads, self.scale, self.window or 0, batch)
         elif batch.is_decode and rt.dtype == torch.bfloat16:
             chunk = decode_chunk(batch.n_seqs, self.num_kv_heads, batch.max_context, self.head_dim)
