@@ -10,8 +10,8 @@
 // a list of pages: those in common, then the tokens' own, each once for the tokens that have it. The list is cut into
 // `splits` stretches of equal length, a block each, so that the device is filled whatever the contexts are; running maximum
 // and sum are kept in float32. Up to eight blocks form a cluster and add their results up through distributed shared memory; where there
-// are more clusters, theirs go to scratch and the block that finishes last for its tile and kv head (a ticket; nobody
-// waits) joins them in order.
+// are more clusters, theirs go to scratch, and of the blocks that have written the same pieces of it the last (a ticket;
+// nobody waits) joins them in order.
 //
 // bfloat16, head sizes that are multiples of 16: from 64 to 128 on the 5th-generation tensor cores (namespace t5), below
 // with mma.sync (mma_kernel). Probabilities are rounded to bfloat16 as the second product's operand. Everything else
@@ -37,9 +37,10 @@ struct Args {
   KvLayout cache;
   const int *slots, *positions, *cuts, *shared;
   float* scratch;      // [tile, kv head][cluster][ROWS][head_dim], then [..][ROWS][2]
-  unsigned* tickets;   // one a (tile, kv head), zero between launches
+  unsigned* tickets;   // one a (tile, kv head) and block of a cluster, zero between launches
   int* status;
   int heads, window, tiles, splits, cluster;  // blocks of a tile and kv head; of a cluster
+  int tokens, max_rows;
   float scale;
 };
 
@@ -65,8 +66,20 @@ __device__ __forceinline__ void make_plan(Plan& p, const Args& a, int rows_per_t
   const int per_kv = a.heads / a.cache.kv_heads;
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
+    constexpr int EACH = MAX_ROWS / 32;
+    const int row0 = tile * rows_per_tile, t0 = row0 / per_kv;
+    // Groups mostly have all the same number of tokens: where this one's would lie then is asked for beside the cuts.
+    const int guess = group * a.max_rows;
+    int pos[EACH], slot[EACH];
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) {
+      const int t = guess + t0 + lane + 32 * u;
+      const bool there = lane + 32 * u < a.max_rows && t < a.tokens;
+      pos[u] = there ? a.positions[t] : -1;
+      slot[u] = there ? a.slots[t] : -1;
+    }
     const int first = a.cuts[group], count = a.cuts[group + 1] - first, shared = a.shared[group];
-    const int row0 = tile * rows_per_tile, rows = min(rows_per_tile, count * per_kv - row0);
+    const int rows = min(rows_per_tile, count * per_kv - row0);
     if (lane == 0) {
       if (tile == a.tiles - 1 && count * per_kv > a.tiles * rows_per_tile)
         *reinterpret_cast<volatile int*>(a.status) = TOO_MANY;  // (the launch was made for fewer tokens a group)
@@ -74,15 +87,18 @@ __device__ __forceinline__ void make_plan(Plan& p, const Args& a, int rows_per_t
       p.total = 0;
     }
     if (rows > 0) {
-      const int t0 = row0 / per_kv, tokens = (row0 + rows - 1) / per_kv - t0 + 1;
-      constexpr int EACH = MAX_ROWS / 32;
+      const int tokens = (row0 + rows - 1) / per_kv - t0 + 1;
       int furthest = -1, which = 0, least_first = FULL, from = 0, to = FULL;
-      int pos[EACH], low[EACH], pages[EACH], slot[EACH];
+      int low[EACH], pages[EACH];
 #pragma unroll
       for (int u = 0; u < EACH; ++u) {
         const int t = lane + 32 * u;
-        pos[u] = t < tokens ? a.positions[first + t0 + t] : -1;
-        slot[u] = t < tokens ? a.slots[first + t0 + t] : -1;
+        if (first != guess || t >= a.max_rows) {
+          pos[u] = t < tokens ? a.positions[first + t0 + t] : -1;
+          slot[u] = t < tokens ? a.slots[first + t0 + t] : -1;
+        } else if (t >= tokens) {
+          pos[u] = slot[u] = -1;
+        }
       }
 #pragma unroll
       for (int u = 0; u < EACH; ++u) {
@@ -258,7 +274,7 @@ __device__ __forceinline__ void write_out(const Plan& p, const Args& a, int r, i
 // Every block has its result in shared memory: x[row * ld ..] sums, ml[row] (maximum, sum); a block without pages has (-inf, 0)
 // there and anything in x. The blocks of the cluster take the rows' pieces in turn. All threads call.
 template <typename T, int ROWS>
-__device__ __forceinline__ void finish(Plan& p, const Args& a, const float* x, int ld, const float2* ml, float* weight) {
+__device__ __forceinline__ void finish(Plan& p, const Args& a, const float* x, int ld, const float2* ml) {
   const int hd = a.cache.head_dim, fours = hd / 4, clusters = a.splits / a.cluster;
   const unsigned size = a.cluster, rank = blockIdx.x % size;
   const size_t pair = (size_t)blockIdx.z * gridDim.y + blockIdx.y;
@@ -308,36 +324,43 @@ __device__ __forceinline__ void finish(Plan& p, const Args& a, const float* x, i
   }
   if (size > 1) cluster_sync();  // nobody leaves while others read its result
   if (clusters == 1) return;
+  // Blocks of one rank have written the same pieces, one cluster's part each: the last of them joins these, in order.
   __syncthreads();
   if (threadIdx.x == 0) {
+    unsigned* ticket = a.tickets + pair * size + rank;
     __threadfence();  // (what the block has written, which the barrier has shown to this thread, before the ticket)
-    p.last = atomicAdd(&a.tickets[pair], 1u) == (unsigned)(a.splits - 1);
+    p.last = atomicAdd(ticket, 1u) == (unsigned)(clusters - 1);
     __threadfence();
-    if (p.last) a.tickets[pair] = 0u;
+    if (p.last) *ticket = 0u;
   }
   __syncthreads();
   if (!p.last) return;
-  // the last block: what each cluster's part counts [cluster][row], then the rows' sums
-  float2* all_ml = reinterpret_cast<float2*>(weight);
-  for (int i = threadIdx.x; i < clusters * ROWS; i += blockDim.x)
-    if (i % ROWS < p.rows) all_ml[i] = __ldcg(reinterpret_cast<const float2*>(part_ml) + pair * clusters * ROWS + i);
-  __syncthreads();
-  for (int i = threadIdx.x; i < p.rows * fours; i += blockDim.x) {
+  for (int i = rank * blockDim.x + threadIdx.x; i < p.rows * fours; i += size * blockDim.x) {
     const int r = i / fours, d = (i % fours) * 4;
     float top = -INFINITY, total = 0.f;
-    for (int c = 0; c < clusters; ++c) top = fmaxf(top, all_ml[c * ROWS + r].x);
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c0 = 0; c0 < clusters; c0 += 4) {
-      float4 v[4];
+    for (int c0 = 0; c0 < clusters; c0 += MAX_CLUSTER) {  // (eight parts at a time, the sum so far faded to the new maximum)
+      float2 each[MAX_CLUSTER];
+      float4 v[MAX_CLUSTER];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (c0 + u < clusters) v[u] = __ldcg(reinterpret_cast<const float4*>(parts + ((pair * clusters + c0 + u) * ROWS + r) * hd + d));
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < MAX_CLUSTER; ++u)
         if (c0 + u < clusters) {
-          const float2 each = all_ml[(c0 + u) * ROWS + r];
-          const float w = share_of(each.x, top);
-          total += each.x > -INFINITY ? w * each.y : each.y;
+          const size_t at = (pair * clusters + c0 + u) * ROWS + r;
+          each[u] = __ldcg(reinterpret_cast<const float2*>(part_ml + at * 2));
+          v[u] = __ldcg(reinterpret_cast<const float4*>(parts + at * hd + d));
+        }
+      const float before = top;
+#pragma unroll
+      for (int u = 0; u < MAX_CLUSTER; ++u)
+        if (c0 + u < clusters) top = fmaxf(top, each[u].x);
+      const float fade = before > -INFINITY ? exp2f(before - top) : 1.f;
+      total *= fade;
+      sum.x *= fade; sum.y *= fade; sum.z *= fade; sum.w *= fade;
+#pragma unroll
+      for (int u = 0; u < MAX_CLUSTER; ++u)
+        if (c0 + u < clusters) {
+          const float w = share_of(each[u].x, top);
+          total += each[u].x > -INFINITY ? w * each[u].y : each[u].y;
           if (w != 0.f) {
             sum.x = fmaf(w, v[u].x, sum.x); sum.y = fmaf(w, v[u].y, sum.y);
             sum.z = fmaf(w, v[u].z, sum.z); sum.w = fmaf(w, v[u].w, sum.w);
@@ -660,7 +683,7 @@ __global__ void __launch_bounds__(WM * 128) mma_kernel(const Args a) {
   } else {
     for (int r = tid; r < ROWS; r += THREADS) sm_ml[r] = make_float2(-INFINITY, 0.f);
   }
-  finish<bf16, ROWS>(p, a, sum, HD, sm_ml, reinterpret_cast<float*>(q_s));
+  finish<bf16, ROWS>(p, a, sum, HD, sm_ml);
 }
 
 template <typename Kernel, typename... Rest>
@@ -1156,13 +1179,12 @@ __global__ void __launch_bounds__(Shape<BOXES, ROWS>::THREADS, 1)
   __syncthreads();
   if (warp == SOFT_WARPS + 1) tmem_dealloc(tmem_base_s, S::COLUMNS);
   if (p.rows == 0) return;
-  finish<bf16, ROWS>(p, a, ex, S::LD, sm_ml, reinterpret_cast<float*>(q_s));
+  finish<bf16, ROWS>(p, a, ex, S::LD, sm_ml);
 }
 
 template <int BOXES, int ROWS>
 int launch(const Args& a, long long pages, dim3 grid, cudaStream_t stream) {
   typedef Shape<BOXES, ROWS> S;
-  static_assert(MAX_CLUSTERS * ROWS * 8 + 1024 <= S::SMEM, "what the join keeps");
   CUtensorMap map;
   if (!make_map(&map, a.cache.base, pages * 2 * a.cache.kv_heads * PAGE, a.cache.head_dim, PAGE)) return DLLM_LAUNCH_FAILED;
   static std::atomic<unsigned long long> done{0};
@@ -1353,7 +1375,7 @@ __global__ void __launch_bounds__(FMA_THREADS) fma_kernel(const Args a) {
   } else {
     if (tid < FMA_ROWS) sm_ml[tid] = make_float2(-INFINITY, 0.f);
   }
-  finish<T, FMA_ROWS>(p, a, q_s, ld, sm_ml, groups_s);
+  finish<T, FMA_ROWS>(p, a, q_s, ld, sm_ml);
 }
 
 // ---- launch shapes -------------------------------------------------------------------------------------------------
@@ -1399,9 +1421,7 @@ template <int HD, int MT, int WM, int STAGES>
 int launch_mma(const Args& a, dim3 grid, cudaStream_t stream) {
   constexpr int ROWS = 16 * MT * WM;
   constexpr int ring = STAGES * 2 * 64 * HD * 2, sums = 4 * ROWS * HD * 4;
-  constexpr int weights = MAX_CLUSTERS * ROWS * 8;
-  constexpr int bytes = ROWS * HD * 2 + (ring > sums ? ring : sums);
-  constexpr int smem = bytes > weights ? bytes : weights;
+  constexpr int smem = ROWS * HD * 2 + (ring > sums ? ring : sums);
   static std::atomic<unsigned long long> done{0};
   if (!dllm_allow_shared((const void*)mma_kernel<HD, MT, WM, STAGES>, smem, done)) return DLLM_LAUNCH_FAILED;
   return launch_clusters(mma_kernel<HD, MT, WM, STAGES>, grid, WM * 128, smem, a.cluster, stream, a);
@@ -1412,16 +1432,15 @@ int launch_fma(const Args& a, dim3 grid, cudaStream_t stream) {
   const int hd = a.cache.head_dim, rows = FMA_ROWS * (hd + 4) * 4;
   const int ring = fma_stages<T>(hd) * 2 * PAGE * fma_row<T>(hd) * (int)sizeof(T);
   const int each = hd, n = FMA_THREADS / each < 16 ? FMA_THREADS / each : 16;  // (groups of keys, of hd / 4 x 4 threads)
-  const int sums = n * FMA_ROWS * (hd + 4) * 4, weights = MAX_CLUSTERS * FMA_ROWS * 8;
-  const int most = ring > sums ? ring : sums;
+  const int sums = n * FMA_ROWS * (hd + 4) * 4;
   static std::atomic<unsigned long long> done{0};
   if (!dllm_allow_shared((const void*)fma_kernel<T>, FMA_MOST, done)) return DLLM_LAUNCH_FAILED;
-  return launch_clusters(fma_kernel<T>, grid, FMA_THREADS, rows + (most > weights ? most : weights), a.cluster, stream, a);
+  return launch_clusters(fma_kernel<T>, grid, FMA_THREADS, rows + (ring > sums ? ring : sums), a.cluster, stream, a);
 }
 }  // namespace
 
 // Query rows of a tile in the low 16 bits, clusters above: scratch holds groups x tiles x kv_heads x clusters x rows x
-// (head_dim + 2) floats where there is more than one, tickets groups x tiles x kv_heads words.
+// (head_dim + 2) floats where there is more than one, tickets groups x tiles x kv_heads x 8 words.
 DLLM_EXPORT int dllm_attention_shared_shape(int dtype, int heads, int kv_heads, int head_dim, int groups, int max_rows,
                                             int max_context) {
   if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || groups <= 0 || max_rows <= 0 || max_context <= 0) return DLLM_BAD_ARGUMENT;
@@ -1432,7 +1451,7 @@ DLLM_EXPORT int dllm_attention_shared_shape(int dtype, int heads, int kv_heads, 
 // See the head of the file. out, q [tokens, heads * head_dim] in the cache's type; slots, positions: each token's table row and
 // position; cuts [groups + 1]: the groups' first tokens; shared [groups]: pages from the first on that a group's table rows have
 // in common; the cache entry has `pages` pages.
-DLLM_EXPORT int dllm_attention_shared(void* out, const void* q, void* base, long long pages, const int* page_table,
+DLLM_EXPORT int dllm_attention_shared(void* out, const void* q, int tokens, void* base, long long pages, const int* page_table,
                                       int max_pages, int page_size, int dtype, int heads, int kv_heads, int head_dim,
                                       const int* slots, const int* positions, const int* cuts, const int* shared, int groups,
                                       int max_rows, int max_context, float scale, int window, float* scratch, unsigned* tickets,
@@ -1445,7 +1464,7 @@ DLLM_EXPORT int dllm_attention_shared(void* out, const void* q, void* base, long
   Shape s = shape_of(dtype, heads, kv_heads, head_dim, groups, max_rows, max_context);
   if ((long long)groups * s.tiles > 65535) return DLLM_UNSUPPORTED_SIZE;
   Args a{out, q, KvLayout{base, page_table, max_pages, page_size, kv_heads, head_dim}, slots, positions, cuts, shared, scratch,
-         tickets, status, heads, window, s.tiles, s.splits, s.cluster, scale};
+         tickets, status, heads, window, s.tiles, s.splits, s.cluster, tokens, max_rows, scale};
   dim3 grid(s.splits, kv_heads, groups * s.tiles);
   if (s.kind == FMA) return dtype == DLLM_BF16 ? launch_fma<bf16>(a, grid, stream) : launch_fma<float>(a, grid, stream);
   if (s.kind == TCGEN05) {

@@ -61,7 +61,7 @@ __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
 
 struct Shared {
   // a stretch's candidates as words that order them (`word_of`); a sequence's as logit and token, total, beam
-  unsigned long long list[LIST];
+  unsigned long long list[LIST], kept[LIST];
   float list_total[LIST];
   int list_beam[LIST];
   float group_max[2][THREADS / 32][MAX_BEAMS];
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(THREADS, 4) select_kernel(const Args a) {
   const int row = blockIdx.y, b = row / a.beams_in, k = row % a.beams_in;
   const int part = blockIdx.x, parts = gridDim.x;
   const int beams = a.beams, vocab = a.vocab;
-  if (tid == 0) sh.list_n = sh.n_ended = sh.seen_n[0] = sh.seen_n[1] = 0;
+  if (tid == 0) sh.list_n = sh.kept_n = sh.n_ended = sh.seen_n[0] = sh.seen_n[1] = 0;
   pdl_launch_dependents();
   pdl_wait();
   // ---- the stretch: whole fours where addresses are multiples of 16 bytes; the up to three logits before and behind those are
@@ -168,12 +168,20 @@ __global__ void __launch_bounds__(THREADS, 4) select_kernel(const Args a) {
   const float4* x4 = reinterpret_cast<const float4*>(x + first);
   float v[4 * REG];
   auto load = [&](int tile) {
+    const int at0 = tile * REG * THREADS + tid;
+    if ((tile + 1) * REG * THREADS <= fours) {
 #pragma unroll
-    for (int r = 0; r < REG; ++r) {
-      float4 four = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-      const int at = (tile * REG + r) * THREADS + tid;
-      if (at < fours) four = __ldcs(x4 + at);
-      v[4 * r] = four.x; v[4 * r + 1] = four.y; v[4 * r + 2] = four.z; v[4 * r + 3] = four.w;
+      for (int r = 0; r < REG; ++r) {
+        const float4 four = __ldcs(x4 + at0 + r * THREADS);
+        v[4 * r] = four.x; v[4 * r + 1] = four.y; v[4 * r + 2] = four.z; v[4 * r + 3] = four.w;
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < REG; ++r) {
+        float4 four = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (at0 + r * THREADS < fours) four = __ldcs(x4 + at0 + r * THREADS);
+        v[4 * r] = four.x; v[4 * r + 1] = four.y; v[4 * r + 2] = four.z; v[4 * r + 3] = four.w;
+      }
     }
   };
   load(0);
@@ -249,32 +257,26 @@ __global__ void __launch_bounds__(THREADS, 4) select_kernel(const Args a) {
       const float m_new = fmaxf(m, top), shift = m_new > -INFINITY ? -m_new : 0.f;
       Two sums[2] = {two(0.f, 0.f), two(0.f, 0.f)};
       const Two shift2 = two(shift, shift), log2e2 = two(LOG2E, LOG2E);
-      unsigned hits = 0u;  // which of this thread's logits reach the bound
 #pragma unroll
-      for (int r = 0; r < REG; ++r) {
-        const float* four = v + 4 * r;
-        if (fmaxf(fmaxf(four[0], four[1]), fmaxf(four[2], four[3])) >= floor_) {
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (four[u] >= floor_) hits |= 1u << (4 * r + u);
-        }
-        // (the difference first: it is exact where the weight is large)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const float2 y = apart(mul2(add2(two(four[2 * u], four[2 * u + 1]), shift2), log2e2));
-          sums[u] = add2(sums[u], two(fast_exp2(y.x), fast_exp2(y.y)));
-        }
+      for (int e = 0; e < 4 * REG; e += 2) {  // (the difference first: it is exact where the weight is large)
+        const float2 y = apart(mul2(add2(two(v[e], v[e + 1]), shift2), log2e2));
+        sums[e >> 1 & 1] = add2(sums[e >> 1 & 1], two(fast_exp2(y.x), fast_exp2(y.y)));
       }
       const float2 all_four = apart(add2(sums[0], sums[1]));
       sum = sum * (m > -INFINITY ? fast_exp2((m + shift) * LOG2E) : 1.f) + (all_four.x + all_four.y);
       m = m_new;
-      while (hits) {
-        const int e = __ffs(hits) - 1;
-        hits &= hits - 1;
-        float value = v[0];
+      if (top >= floor_) {  // (few threads of a tile have something that reaches the bound)
+        unsigned hits = 0u;
 #pragma unroll
-        for (int j = 1; j < 4 * REG; ++j) value = e == j ? v[j] : value;
-        offer(value, place_of(tile, e));
+        for (int e = 0; e < 4 * REG; ++e) hits |= v[e] >= floor_ ? 1u << e : 0u;
+        while (hits) {
+          const int e = __ffs(hits) - 1;
+          hits &= hits - 1;
+          float value = v[0];
+#pragma unroll
+          for (int j = 1; j < 4 * REG; ++j) value = e == j ? v[j] : value;
+          offer(value, place_of(tile, e));
+        }
       }
     }
     if (extra >= fmaxf(low, -FLT_MAX)) offer(extra, extra_at);
@@ -293,16 +295,27 @@ __global__ void __launch_bounds__(THREADS, 4) select_kernel(const Args a) {
     }
     const int n = sh.list_n;
     if (n <= LIST) {
-      for (int c = tid; c < n; c += THREADS) {
-        const unsigned long long mine_word = sh.list[c];
-        if (logit_of(mine_word) < low) continue;  // (in the list by an earlier bound)
+      // what reaches the bound of all tiles (all of it, where that is -inf), in order: each counts what is before it
+      const unsigned long long* from = sh.list;
+      int kept = n;
+      if (tiles > 1) {
+        low = bound_of<GROUPS>(keep, sh, updates & 1);
+        const unsigned long long least = word_of(fmaxf(low, -FLT_MAX), 0x7fffffff);
+        for (int c = tid; c < n; c += THREADS)
+          if (sh.list[c] >= least) sh.kept[atomicAdd(&sh.kept_n, 1)] = sh.list[c];
+        __syncthreads();
+        from = sh.kept;
+        kept = sh.kept_n;
+      }
+      for (int c = tid; c < kept; c += THREADS) {
+        const unsigned long long mine_word = from[c];
         int place = 0;
 #pragma unroll 8
-        for (int j = 0; j < n; ++j) place += sh.list[j] > mine_word ? 1 : 0;
+        for (int j = 0; j < kept; ++j) place += from[j] > mine_word ? 1 : 0;
         if (place < beams) { mine[2 + 2 * place] = logit_of(mine_word); mine[3 + 2 * place] = __int_as_float(token_of(mine_word)); }
       }
-      // (fewer than `beams` that may be chosen: all of them are in the list, whatever the bound)
-      for (int c = n + tid; c < beams; c += THREADS) { mine[2 + 2 * c] = -INFINITY; mine[3 + 2 * c] = 0.f; }
+      // (fewer than `beams` that may be chosen: all of them are there, the bound is -inf)
+      for (int c = kept + tid; c < beams; c += THREADS) { mine[2 + 2 * c] = -INFINITY; mine[3 + 2 * c] = 0.f; }
     } else {
       // one after another: the best that comes behind the last one. (A word orders by logit, then by the lower token.)
       unsigned long long last = ~0ull;

@@ -4,6 +4,7 @@ no CPU path and no library fallback: a tensor that is not on a CUDA device is an
 from __future__ import annotations
 
 import ctypes
+import functools
 from ctypes import c_double, c_float, c_int, c_longlong, c_void_p
 
 import torch
@@ -262,7 +263,7 @@ _prototypes = {
                                           c_int, c_void_p],
     ("attention_shared", "dllm_attention_shared_shape"): [c_int, c_int, c_int, c_int, c_int, c_int, c_int],
     ("attention_shared", "dllm_attention_shared"): [
-        c_void_p, c_void_p, c_void_p, c_longlong, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+        c_void_p, c_void_p, c_int, c_void_p, c_longlong, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
         c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
     ("beam_reorder", "dllm_beam_reorder"): [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                             c_void_p],
@@ -2263,13 +2264,18 @@ MAX_BEAMS, MAX_BEAM_STOPS = 32, 8
 """The most beams of a sequence, and the most stop tokens, that a beam search takes."""
 
 
+@functools.lru_cache(maxsize=1024)
+def _beam_select_parts(rows: int, vocab: int) -> int:
+    parts = _fn("beam_select", "dllm_beam_select_parts")(rows, vocab)
+    if parts <= 0:
+        raise KernelError(f"beam_select: {_STATUS.get(parts, parts)} ({rows} rows of {vocab})")
+    return parts
+
+
 def beam_select_scratch(sequences: int, beams_in: int, vocab: int, beams: int) -> int:
     """Floats of scratch that `beam_select` needs."""
     rows = sequences * beams_in
-    parts = _fn("beam_select", "dllm_beam_select_parts")(rows, vocab)
-    if parts <= 0:
-        raise KernelError(f"beam_select: {_STATUS.get(parts, parts)}")
-    return rows * parts * (2 + 2 * beams)
+    return rows * _beam_select_parts(rows, vocab) * (2 + 2 * beams)
 
 
 def beam_select(parents: torch.Tensor, tokens: torch.Tensor, out: tuple, logits: torch.Tensor, state: tuple,
@@ -2293,7 +2299,8 @@ def beam_select(parents: torch.Tensor, tokens: torch.Tensor, out: tuple, logits:
     _cuda(parents, tokens, logits, scores, finished, finished_at, done, scores_out, finished_out, finished_at_out, done_out,
           produced, scratch, tickets, stop_ids, steps, history)
     sequences, beams_in = scores.shape
-    beams, vocab = parents.shape[1], logits.shape[1]
+    n, beams = parents.shape
+    rows, vocab = logits.shape
     if not 0 < beams <= MAX_BEAMS or not 0 < beams_in <= MAX_BEAMS:
         raise KernelError(f"beam_select: {beams_in} beams to {beams}: 1 to {MAX_BEAMS}")
     stops = stop_ids.numel() if stop_ids is not None else 0
@@ -2305,23 +2312,23 @@ def beam_select(parents: torch.Tensor, tokens: torch.Tensor, out: tuple, logits:
             and finished_at.dtype is i32 and finished_at_out.dtype is i32 and done.dtype is i32 and done_out.dtype is i32
             and produced.dtype is i32 and tickets.dtype is i32):
         raise KernelError("beam_select: logits, scores, finished and scratch are float32, all else int32")
-    if not (logits.shape[0] == sequences * beams_in and parents.shape[0] == sequences and tokens.numel() == parents.numel()
-            and scores_out.numel() == finished.numel() == finished_out.numel() == sequences * beams
-            and finished_at.numel() == finished_at_out.numel() == 2 * sequences * beams
+    places = sequences * beams
+    if not (rows == sequences * beams_in and n == sequences and tokens.numel() == scores_out.numel() == finished.numel() == places
+            and finished_out.numel() == places and finished_at.numel() == finished_at_out.numel() == 2 * places
             and done.numel() == done_out.numel() == sequences and tickets.numel() >= sequences):
         raise KernelError(f"beam_select: logits {tuple(logits.shape)}, scores {tuple(scores.shape)} and {beams} beams do not "
                           f"go together with the shapes of the rest")
-    if scratch.numel() < beam_select_scratch(sequences, beams_in, vocab, beams) or scratch.data_ptr() % 8:
+    at = scratch.data_ptr()
+    if scratch.numel() < rows * _beam_select_parts(rows, vocab) * (2 + 2 * beams) or at % 8:
         raise KernelError("beam_select: scratch is too small (beam_select_scratch) or not aligned to 8 bytes")
     if (stops and stop_ids.dtype is not i32) or (steps is not None and steps.dtype is not i32) or (
-            history is not None and (history.dtype is not i32 or history.numel() % (sequences * beams) or steps is None)):
+            history is not None and (history.dtype is not i32 or history.numel() % places or steps is None)):
         raise KernelError("beam_select: stop_ids, steps and history are int32; history [capacity, sequences, beams] needs steps")
     _check(_fn("beam_select", "dllm_beam_select")(
-        logits.data_ptr(), logits.stride(0), scores.data_ptr(), finished.data_ptr(), finished_at.data_ptr(), done.data_ptr(),
-        produced.data_ptr(), steps.data_ptr() if steps is not None else None, stop_ids.data_ptr() if stops else None, stops,
+        logits.data_ptr(), vocab, scores.data_ptr(), finished.data_ptr(), finished_at.data_ptr(), done.data_ptr(), produced.data_ptr(), steps.data_ptr() if steps is not None else None, stop_ids.data_ptr() if stops else None, stops,
         scores_out.data_ptr(), finished_out.data_ptr(), finished_at_out.data_ptr(), done_out.data_ptr(), parents.data_ptr(),
         tokens.data_ptr(), history.data_ptr() if history is not None else None,
-        history.numel() // (sequences * beams) if history is not None else 0, scratch.data_ptr(), tickets.data_ptr(),
+        history.numel() // places if history is not None else 0, at, tickets.data_ptr(),
         sequences, beams_in, beams, vocab, int(min_tokens), float(length_penalty), int(bool(early)), _stream()),
         "beam_select", lambda: f"{sequences} sequences of {beams_in} beams: at most 65,535 rows")
 
@@ -2395,16 +2402,20 @@ def attention_shared_supported(cache) -> bool:
         and cache.value_dim == cache.head_dim and not cache.keys_only
 
 
+@functools.lru_cache(maxsize=1024)
+def _shared_shape(code: int, heads: int, kv_heads: int, head_dim: int, groups: int, max_rows: int, max_context: int) -> tuple[int, int]:
+    shape = _fn("attention_shared", "dllm_attention_shared_shape")(code, heads, kv_heads, head_dim, groups, max_rows, max_context)
+    if shape <= 0:
+        raise KernelError(f"attention_shared: {_STATUS.get(shape, shape)} ({heads} heads on {kv_heads}, {groups} groups of "
+                          f"{max_rows}, contexts of {max_context})")
+    rows, clusters = shape & 0xFFFF, shape >> 16
+    pairs = groups * -(-max_rows * (heads // kv_heads) // rows) * kv_heads
+    return (pairs * clusters * rows * (head_dim + 2), 8 * pairs) if clusters > 1 else (0, 0)
+
+
 def attention_shared_scratch(cache, heads: int, groups: int, max_rows: int, max_context: int) -> tuple[int, int]:
     """(floats of scratch, int32 tickets) that `attention_shared` needs for these bounds."""
-    shape = _fn("attention_shared", "dllm_attention_shared_shape")(
-        _code(cache.dtype), heads, cache.kv_heads, cache.head_dim, groups, max_rows, max_context)
-    if shape <= 0:
-        raise KernelError(f"attention_shared: {_STATUS.get(shape, shape)} ({heads} heads on {cache.kv_heads}, {groups} groups "
-                          f"of {max_rows}, contexts of {max_context})")
-    rows, splits = shape & 0xFFFF, shape >> 16
-    pairs = groups * -(-max_rows * (heads // cache.kv_heads) // rows) * cache.kv_heads
-    return (pairs * splits * rows * (cache.head_dim + 2) if splits > 1 else 0), pairs
+    return _shared_shape(_code(cache.dtype), heads, cache.kv_heads, cache.head_dim, groups, max_rows, max_context)
 
 
 def attention_shared(out: torch.Tensor, q: torch.Tensor, cache, heads: int, scale: float, window: int, slots: torch.Tensor,
@@ -2438,7 +2449,7 @@ def attention_shared(out: torch.Tensor, q: torch.Tensor, cache, heads: int, scal
     if max_context > cache.max_pages * cache.page_size:
         raise KernelError(f"attention_shared: contexts of {max_context} in table rows of {cache.max_pages} pages")
     _check(_fn("attention_shared", "dllm_attention_shared")(
-        out.data_ptr(), q.data_ptr(), cache.base_ptr, cache.storage.shape[0], cache.page_table.data_ptr(), cache.max_pages, cache.page_size,
+        out.data_ptr(), q.data_ptr(), tokens, cache.base_ptr, cache.storage.shape[0], cache.page_table.data_ptr(), cache.max_pages, cache.page_size,
         _code(cache.dtype), heads, cache.kv_heads, cache.head_dim, slots.data_ptr(), positions.data_ptr(), groups.data_ptr(),
         shared.data_ptr(), count, max_rows, max_context, float(scale), int(window or 0), scratch.data_ptr(), tickets.data_ptr(),
         _status_word().data_ptr(), _stream()), "attention_shared",

@@ -543,10 +543,17 @@ def test_attention_refusals():
                          (dict(dtype=torch.float16), "float16"), (dict(heads=3), "heads"), (dict(q=bad), "q torch.float32"),
                          (dict(out=torch.zeros((1, 256), dtype=torch.bfloat16, device=DEV)), "out"), (dict(slots=_i32([0])), "slots"),
                          (dict(positions=_i32([3, 4]).long()), "int32"), (dict(scratch=torch.zeros(64, device=DEV, dtype=torch.float64)), "float32"),
-                         (dict(tickets=_i32([0])), "tickets"), (dict(max_context=200), "table rows"), (dict(max_rows=0), "unsupported|argument"),
+                         (dict(max_context=200), "table rows"), (dict(max_rows=0), "unsupported|argument"),
                          (dict(q=torch.zeros((2, 256), dtype=torch.bfloat16)), "CUDA")]:
         with pytest.raises(o.KernelError, match=says):
             call(**change)
+    long = Pages("chunk", [(0, [9000, 9001])], 4, 2, 64, torch.bfloat16)
+    view = KvView(long.storage.to(DEV), long.table.to(DEV), 64, 2, 64, None)
+    floats, words = o.attention_shared_scratch(view, 4, 1, 2, 9002)
+    for scratch, tickets in ((floats - 1, words), (floats, words - 1)):
+        with pytest.raises(o.KernelError, match="tickets"):
+            o.attention_shared(long.q.to(DEV), long.q.to(DEV), view, 4, 0.1, 0, _i32(long.slots), _i32(long.positions), _i32(long.cuts),
+                               _i32(long.shared), 2, 9002, torch.zeros(scratch, device=DEV), torch.zeros(tickets, dtype=torch.int32, device=DEV))
 
 
 # ---- whole searches --------------------------------------------------------------------------------------------------
