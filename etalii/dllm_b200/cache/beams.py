@@ -10,10 +10,12 @@ import torch
 from .allocators import CacheError
 
 _PIECE = np.dtype([("base", "<i8"), ("stride", "<i8"), ("table", "<i8"), ("units", "<i8"), ("table_width", "<i4"),
-                   ("kind", "<i4"), ("bytes", "<i4"), ("vector", "<i4"), ("unused", "<i8", 2)])
+                   ("kind", "<i4"), ("bytes", "<i4"), ("vector", "<i4"), ("first", "<i4"), ("count", "<i4"), ("unused", "<i8")])
 _ROWS, _STATE, _TABLE = 0, 1, 2
-STATE_PIECE = 16 << 10
+STATE_PIECE = 8 << 10
 """Bytes of a state that one block moves."""
+ROWS_PIECE = 32
+"""Rows of a plane that one block moves."""
 
 
 def _vector(*numbers: int) -> int:
@@ -48,10 +50,12 @@ class CacheRows:
             entries, n_pages, size = storage.shape[0], storage.shape[1], storage.element_size()
             for dim, behind in ((key_dim, 0), (value_dim, kv_heads * self.page_size * key_dim)):
                 if dim:
-                    piece = np.zeros((entries, kv_heads), _PIECE)
-                    piece["base"] = (storage.data_ptr() + size * behind
-                                     + np.arange(entries, dtype=np.int64)[:, None] * (n_pages * per_page * size)
-                                     + np.arange(kv_heads, dtype=np.int64)[None, :] * (self.page_size * dim * size))
+                    first = np.arange(0, self.page_size, ROWS_PIECE, dtype=np.int64)
+                    piece = np.zeros((entries, kv_heads, len(first)), _PIECE)
+                    piece["base"] = (storage.data_ptr() + size * behind + first[None, None, :] * (dim * size)
+                                     + np.arange(entries, dtype=np.int64)[:, None, None] * (n_pages * per_page * size)
+                                     + np.arange(kv_heads, dtype=np.int64)[None, :, None] * (self.page_size * dim * size))
+                    piece["first"], piece["count"] = first, np.minimum(ROWS_PIECE, self.page_size - first)
                     piece["stride"], piece["units"] = per_page * size, n_pages
                     piece["table"], piece["table_width"] = table.data_ptr(), table.shape[1]
                     piece["kind"], piece["bytes"] = _ROWS, dim * size

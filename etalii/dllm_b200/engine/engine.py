@@ -64,7 +64,7 @@ class Engine:
         `decode_logits`: decode runs always compute the logits (they stay readable in the run's buffer); by default
         a greedy run lets the head product choose the token itself and stores no logits. `split_chunks`: steps in which
         sequences bring at most this many new tokens (and one of them more than one) cut their contexts' keys over the
-        device (`ops.attention_shared`), where the parts can: for a few tokens appended to long contexts. 0: never."""
+        device (`ops.attention_shared`), where the parts can and contexts are long enough to gain. 0: never."""
         if not torch.cuda.is_available():
             raise RuntimeError("no CUDA device: this library has no CPU path")
         self.config = config

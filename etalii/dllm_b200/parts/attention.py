@@ -34,6 +34,30 @@ from about 768 keys per query on, 1.3 to 1.6 times at 2,048 and more, while on s
 weigh more and the mma.sync kernel with its tiles of 64 queries is as fast or a little faster."""
 
 
+SHARED_FROM_BYTES = {torch.float32: (64 << 20, 64 << 20), torch.bfloat16: (128 << 20, 32 << 20)}
+SHARED_FROM_CONTEXT = 768
+
+
+def reads_shared_pages(batch, cache) -> bool:
+    """Whether a step whose tokens share pages (`batch.shared`) attends with `ops.attention_shared`: it costs 9 to 12 µs
+    whatever the contexts are, where the kernels that read every token's pages cost 3 to 10 µs and then grow with them. Beams: from
+    so many bytes of keys and values on, counted for every beam (heads up to 64, above; and 1 MB for every prompt and kv head: their
+    blocks take turns). Short chunks: from 768 positions on. Measured, µs, shared and not: 8 x 8 beams, 9 heads on 3 of 64,
+    1,000 positions 12.3 and 8.8, 4,000 16.2 and 20.3; 32 heads on 8 of 128, 500 positions 16.4 and 28.1, 4,000 32.7 and 102.5; 1 x 4, 2,000
+    positions 13.0 and 9.2, 4,000 15.0 and 15.3; float32, 9 heads on 3 of 64, 8 x 8 beams on 250 positions 21.1 and 17.8, on 2,000 49.9 and
+    106.6; eight new tokens on 250, 1,000 and 16,000 positions, 32 heads on 8 of 128, 10.0 and 9.3, 10.2 and 16.3, 23.4 and 166.9."""
+    shared = getattr(batch, "shared", None)
+    if shared is None or not ops.attention_shared_supported(cache):
+        return False
+    if not batch.is_decode:
+        return batch.max_context >= SHARED_FROM_CONTEXT
+    if cache.dtype == torch.bfloat16 and not ops.attention_decode_cluster_supported(cache):
+        return True  # (heads that the cluster kernel does not take)
+    per_position = 2 * cache.kv_heads * cache.head_dim * cache.storage.element_size()
+    least = SHARED_FROM_BYTES[cache.dtype][1 if cache.head_dim > 64 else 0]
+    return batch.n_tokens * batch.max_context * per_position >= max(least, (shared.groups.numel() - 1) * cache.kv_heads << 20)
+
+
 class Attention:
     accepts_pending_norm = True
 
@@ -156,9 +180,9 @@ class Attention:
                    out_scale=self.output_scale, out_at=at)
             return
         attended = rt.ws.buffer("attended", (n, q_size), rt.dtype)
-        shared = getattr(batch, "shared", None)
-        if shared is not None and ops.attention_shared_supported(cache):
+        if reads_shared_pages(batch, cache):
             # beams, or a few tokens appended to each sequence: pages in common are read once
+            shared = batch.shared
             longest = min(batch.max_context, cache.max_pages * cache.page_size)
             floats, tickets = ops.attention_shared_scratch(cache, self.num_heads, shared.groups.numel() - 1, shared.max_rows, longest)
             ops.attention_shared(attended, q, cache, self.num_heads, self.scale, self.window or 0, shared.slots, batch.tok_pos,

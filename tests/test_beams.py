@@ -114,13 +114,16 @@ def test_the_list_of_what_beams_move():
     narrow = torch.zeros((6, 3), dtype=torch.float32)
     rows = CacheRows([(storage, table, 3, 16, 8), (only, table, 1, 40, 0)], [state, narrow], 64)
     pieces = rows.pieces.numpy()
-    # 2 entries x 3 heads of keys and of values, a table; 1 x 1 of keys, a table; 20,000 bytes in two pieces; 12 in one
-    assert rows.n_pieces == len(pieces) == 6 + 6 + 1 + 1 + 1 + 2 + 1
+    # 2 entries x 3 heads x 2 halves of keys and of values, a table; 1 x 1 x 2 of keys, a table; 20,000 bytes in three pieces; 12 in one
+    assert rows.n_pieces == len(pieces) == 12 + 12 + 1 + 2 + 1 + 3 + 1
     kinds, sizes = pieces[:, 4] >> 32, pieces[:, 5] & 0xFFFFFFFF
-    assert kinds.tolist() == [0] * 12 + [2, 0, 2, 1, 1, 1]
-    assert sizes[:12].tolist() == [32] * 6 + [16] * 6 and sizes[13] == 160 and sizes[15:].tolist() == [16384, 3616, 12]
-    assert pieces[7, 0] - storage.data_ptr() == 3 * 64 * 16 * 2 + 64 * 8 * 2  # values of head 1 of entry 0
-    assert pieces[9, 0] - pieces[6, 0] == storage[0].numel() * 2 and (pieces[:12, 1] == 3 * 64 * 24 * 2).all()
+    assert kinds.tolist() == [0] * 24 + [2, 0, 0, 2, 1, 1, 1, 1]
+    assert sizes[:24].tolist() == [32] * 12 + [16] * 12 and sizes[25] == 160 and sizes[28:].tolist() == [8192, 8192, 3616, 12]
+    assert pieces[14, 0] - storage.data_ptr() == 3 * 64 * 16 * 2 + 64 * 8 * 2  # values of head 1 of entry 0
+    assert pieces[15, 0] - pieces[14, 0] == 32 * 8 * 2                          # and their other half
+    assert pieces[18, 0] - pieces[12, 0] == storage[0].numel() * 2 and (pieces[:24, 1] == 3 * 64 * 24 * 2).all()
+    first, count = pieces[:24, 6] & 0xFFFFFFFF, pieces[:24, 6] >> 32
+    assert first.tolist() == [0, 32] * 12 and (count == 32).all()
     assert (pieces[-1, 5] >> 32) == 4 and (pieces[0, 5] >> 32) == 16
 
 

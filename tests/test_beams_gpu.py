@@ -588,6 +588,32 @@ def test_search_is_the_plain_search(tag, beams, penalty, early, graphs):
     assert engine.cache.slots.held == 0 and engine.cache.pages_held() == 0
 
 
+@pytest.mark.parametrize("dtype,head_dim", [("float32", 32), ("float32", 64), ("bfloat16", 32), ("bfloat16", 64), ("bfloat16", 72)])
+def test_search_whose_beams_read_shared_pages(dtype, head_dim, monkeypatch):
+    """The same search with the attention that reads pages once and with the one that reads every beam's (what a step takes goes by
+    its size otherwise): the same texts in float32, scores within the rounding of the logits."""
+    from etalii.dllm_b200.parts import attention
+    from etalii.dllm_b200.sampling.beams import BeamOptions
+
+    config, _ = model_case("a")
+    config = {**config, "num_attention_heads": 4, "num_key_value_heads": 2, "head_dim": head_dim, "max_position_embeddings": 512}
+    weights = P.random_weights(config, 6, std=0.08)
+    prompts = prompts_for(config, [20, 128, 200])
+    found = []
+    for least in (0, 1 << 60):
+        monkeypatch.setattr(attention, "SHARED_FROM_BYTES", {d: (least, least) for d in attention.SHARED_FROM_BYTES})
+        monkeypatch.setattr(attention, "reads_shared_pages",
+                            lambda batch, cache, least=least: getattr(batch, "shared", None) is not None and least == 0)
+        engine = make_engine(config, weights, dtype, max_tokens=4096)
+        before = ops().launches
+        found.append(engine.beam_search(prompts, 70, BeamOptions(beams=3), ignore_eos=True))
+        assert ops().launches > before
+    for one, other in zip(*found):
+        if dtype == "float32":
+            assert [r.tokens for r in one] == [r.tokens for r in other]
+        assert abs(one[0].score - other[0].score) <= (1e-3 if dtype == "float32" else 0.06)
+
+
 def test_one_beam_is_the_greedy_choice():
     from etalii.dllm_b200.sampling.beams import BeamOptions
 
@@ -681,7 +707,7 @@ def test_short_chunks_over_the_whole_device(dtype, tolerance):
     config = {**config, "num_attention_heads": 2, "num_key_value_heads": 1, "head_dim": 64, "max_position_embeddings": 2048}
     weights = P.random_weights(config, 5, std=0.08)
     plain, cut = (make_engine(config, weights, dtype, max_tokens=8192, split_chunks=n) for n in (0, 8))
-    prompts = prompts_for(config, [700, 63, 5])
+    prompts = prompts_for(config, [1500, 63, 5])
     outs = []
     for engine in (plain, cut):
         slots = engine.open(3)
