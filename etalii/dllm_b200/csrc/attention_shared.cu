@@ -238,6 +238,11 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n"
                "barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
+// The same without an order of memory: for those that wait until others have read what is theirs.
+__device__ __forceinline__ void cluster_wait_for_readers() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n"
+               "barrier.cluster.wait.aligned;\n" ::: "memory");
+}
 __device__ __forceinline__ unsigned remote_addr(const void* local, unsigned rank) {
   unsigned addr = (unsigned)__cvta_generic_to_shared(local), remote;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
@@ -322,7 +327,7 @@ __device__ __forceinline__ void finish(Plan& p, const Args& a, const float* x, i
       if (d == 0) *reinterpret_cast<float2*>(part_ml + at * 2) = make_float2(top, total);
     }
   }
-  if (size > 1) cluster_sync();  // nobody leaves while others read its result
+  if (size > 1) cluster_wait_for_readers();  // nobody leaves while others read its result
   if (clusters == 1) return;
   // Blocks of one rank have written the same pieces, one cluster's part each: the last of them joins these, in order.
   __syncthreads();
@@ -1139,16 +1144,18 @@ __global__ void __launch_bounds__(Shape<BOXES, ROWS>::THREADS, 1)
 #pragma unroll
       for (int i = 1; i < GROUPS; ++i) most = fmaxf(most, sm_m[i][row]);
       const float w = share_of(m_run, most);
-      const int d = quarter * 32 + lane;
+      const int d = quarter * 32 + lane, active = min(GROUPS, steps);  // (groups that have had a step)
+      if (taken >= 1) {
 #pragma unroll
-      for (int c0 = 0; c0 < 32; c0 += 16) {
-        unsigned o[16];
-        if (taken >= 1) tmem_load16(o_addr + (unsigned)c0, o);
-        float* to = ex + (size_t)(g * ROWS + row0 + c0) * S::LD + d;
+        for (int c0 = 0; c0 < 32; c0 += 16) {
+          unsigned o[16];
+          tmem_load16(o_addr + (unsigned)c0, o);
+          float* to = ex + (size_t)(g * ROWS + row0 + c0) * S::LD + d;
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          const float wc = __shfl_sync(0xffffffffu, w, c0 + c);
-          if (d < BOXES * 64) to[c * S::LD] = taken >= 1 && wc != 0.f ? __uint_as_float(o[c]) * wc : 0.f;
+          for (int c = 0; c < 16; ++c) {
+            const float wc = __shfl_sync(0xffffffffu, w, c0 + c);
+            if (d < BOXES * 64) to[c * S::LD] = wc != 0.f ? __uint_as_float(o[c]) * wc : 0.f;
+          }
         }
       }
       if (g == 0 && quarter == 0) {
@@ -1160,12 +1167,13 @@ __global__ void __launch_bounds__(Shape<BOXES, ROWS>::THREADS, 1)
         }
         sm_ml[row] = make_float2(most, total);
       }
-      asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
-      for (int i = tid; i < ROWS * (BOXES * 16); i += SOFT_WARPS * 32) {  // (into the first group's place)
+      if (active > 1) asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
+      for (int i = active > 1 ? tid : ROWS * (BOXES * 16); i < ROWS * (BOXES * 16); i += SOFT_WARPS * 32) {  // (into the first group's place)
         float4* x = reinterpret_cast<float4*>(ex + (size_t)(i / (BOXES * 16)) * S::LD + (i % (BOXES * 16)) * 4);
         float4 z = *x;
 #pragma unroll
         for (int e = 1; e < GROUPS; ++e) {
+          if (e >= active) break;
           const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(x) + (size_t)e * ROWS * S::LD);
           z.x += y.x; z.y += y.y; z.z += y.z; z.w += y.w;
         }
