@@ -735,13 +735,13 @@ using namespace tc5;
 constexpr int KEYS = 2 * PAGE;
 constexpr int P_BYTES = KEYS * 128;  // [key][64 rows]
 
-template <int BOXES, int ROWS> struct Shape {
-  static constexpr int GROUPS = BOXES == 1 && ROWS == 32 ? 3 : 2;
+template <int BOXES, int ROWS, int GROUPS> struct Shape {
+  static constexpr int BLOCKS = GROUPS == 1 ? 2 : 1;            // of a multiprocessor
   static constexpr int HALVES = ROWS / 32;                      // warps that share a step's keys, 32 rows each
   static constexpr int GROUP = 4 * HALVES, SOFT_WARPS = GROUPS * GROUP, THREADS = (SOFT_WARPS + 3) * 32;
-  static constexpr int K_STAGES = BOXES == 2 ? 2 : 4, V_STAGES = BOXES == 2 ? 3 : 5;
+  static constexpr int K_STAGES = BOXES == 2 || GROUPS == 1 ? 2 : 4, V_STAGES = GROUPS == 1 ? 2 : BOXES == 2 ? 3 : 5;
   static constexpr int Q_BYTES = BOXES * ROWS * 128, KV_BYTES = BOXES * KEYS * 128;
-  static constexpr unsigned COLUMNS = 2 * GROUPS * ROWS > 128 ? 256 : 128;  // of tensor memory: scores and outputs
+  static constexpr unsigned COLUMNS = 2 * GROUPS * ROWS > 128 ? 256 : 2 * GROUPS * ROWS > 64 ? 128 : 64;  // of tensor memory: scores and outputs
   static constexpr int SMEM = Q_BYTES + GROUPS * P_BYTES + (K_STAGES + V_STAGES) * KV_BYTES + 1024;
   static constexpr int LD = BOXES * 64 + 4;  // floats of a row of the results at the end, which lie in the stages' place
   static_assert(GROUPS * ROWS * LD * 4 <= (K_STAGES + V_STAGES) * KV_BYTES, "results");
@@ -789,11 +789,11 @@ __device__ __forceinline__ Two mul2(Two a, Two b) {
   return r;
 }
 
-template <int BOXES, int ROWS>
-__global__ void __launch_bounds__(Shape<BOXES, ROWS>::THREADS, 1)
+template <int BOXES, int ROWS, int GROUPS>
+__global__ void __launch_bounds__(Shape<BOXES, ROWS, GROUPS>::THREADS, Shape<BOXES, ROWS, GROUPS>::BLOCKS)
     kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
-  typedef Shape<BOXES, ROWS> S;
-  constexpr int GROUPS = S::GROUPS, K_STAGES = S::K_STAGES, V_STAGES = S::V_STAGES, KV_BYTES = S::KV_BYTES, SOFT_WARPS = S::SOFT_WARPS;
+  typedef Shape<BOXES, ROWS, GROUPS> S;
+  constexpr int K_STAGES = S::K_STAGES, V_STAGES = S::V_STAGES, KV_BYTES = S::KV_BYTES, SOFT_WARPS = S::SOFT_WARPS;
   constexpr int BOX = KEYS * 128;  // bytes of 64 columns of a step's keys or values
   extern __shared__ __align__(128) unsigned char smem_raw[];
   unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);  // swizzle atoms: 1 KB
@@ -1190,14 +1190,14 @@ __global__ void __launch_bounds__(Shape<BOXES, ROWS>::THREADS, 1)
   finish<bf16, ROWS>(p, a, ex, S::LD, sm_ml);
 }
 
-template <int BOXES, int ROWS>
+template <int BOXES, int ROWS, int GROUPS>
 int launch(const Args& a, long long pages, dim3 grid, cudaStream_t stream) {
-  typedef Shape<BOXES, ROWS> S;
+  typedef Shape<BOXES, ROWS, GROUPS> S;
   CUtensorMap map;
   if (!make_map(&map, a.cache.base, pages * 2 * a.cache.kv_heads * PAGE, a.cache.head_dim, PAGE)) return DLLM_LAUNCH_FAILED;
   static std::atomic<unsigned long long> done{0};
-  if (!dllm_allow_shared((const void*)kernel<BOXES, ROWS>, S::SMEM, done)) return DLLM_LAUNCH_FAILED;
-  return launch_clusters(kernel<BOXES, ROWS>, grid, S::THREADS, S::SMEM, a.cluster, stream, map, a);
+  if (!dllm_allow_shared((const void*)kernel<BOXES, ROWS, GROUPS>, S::SMEM, done)) return DLLM_LAUNCH_FAILED;
+  return launch_clusters(kernel<BOXES, ROWS, GROUPS>, grid, S::THREADS, S::SMEM, a.cluster, stream, map, a);
 }
 }  // namespace t5
 
@@ -1388,7 +1388,7 @@ __global__ void __launch_bounds__(FMA_THREADS) fma_kernel(const Args a) {
 
 // ---- launch shapes -------------------------------------------------------------------------------------------------
 enum { FMA, MMA, TCGEN05 };
-struct Shape { int kind, rows, tiles, splits, cluster; };
+struct Shape { int kind, rows, tiles, splits, cluster; bool several; };  // several: two blocks of a multiprocessor
 
 Shape shape_of(int dtype, int heads, int kv_heads, int head_dim, int groups, int max_rows, int max_context) {
   Shape s;
@@ -1407,11 +1407,12 @@ Shape shape_of(int dtype, int heads, int kv_heads, int head_dim, int groups, int
   // of a part are left over.) Eight new tokens, 32 heads on 8 of 128, us with one cluster of 8, 4 of 4, 9 of 2 and 18 of 1: 2,000 positions
   // 13.4, 17.2, 20.7, 24.1; 80,000: -, 62.6, 65.9, 70.1.
   static const int RESIDENT[2][4] = {{148, 74, 33, 15}, {296, 148, 71, 33}};
-  const int several = s.kind == MMA || (s.kind == FMA && head_dim * (dtype == DLLM_BF16 ? 2 : 4) <= 256);  // (two of a multiprocessor)
   const long long pairs = (long long)groups * s.tiles * kv_heads, most = pages + max_rows;
+  s.several = s.kind == MMA || (s.kind == FMA && head_dim * (dtype == DLLM_BF16 ? 2 : 4) <= 256) ||
+              (s.kind == TCGEN05 && head_dim == 64 && s.rows == 32 && pairs > 148);
   long long blocks[4], best = 0;
   for (int c = 0; c < 4; ++c) {
-    long long n = RESIDENT[several][c] / pairs;
+    long long n = RESIDENT[s.several][c] / pairs;
     if (n > MAX_CLUSTERS) n = MAX_CLUSTERS;
     if (pages <= 64 && n > 1 && c > 0) n = 1;
     if (pages <= 64 && n > 1) n = 0;
@@ -1477,8 +1478,9 @@ DLLM_EXPORT int dllm_attention_shared(void* out, const void* q, int tokens, void
   if (s.kind == FMA) return dtype == DLLM_BF16 ? launch_fma<bf16>(a, grid, stream) : launch_fma<float>(a, grid, stream);
   if (s.kind == TCGEN05) {
     if (pages * 2 * kv_heads * PAGE > 0x7fffffffll) return DLLM_UNSUPPORTED_SIZE;  // (a TMA coordinate is an int)
-    if (head_dim == 64) return s.rows == 32 ? t5::launch<1, 32>(a, pages, grid, stream) : t5::launch<1, 64>(a, pages, grid, stream);
-    return s.rows == 32 ? t5::launch<2, 32>(a, pages, grid, stream) : t5::launch<2, 64>(a, pages, grid, stream);
+    if (head_dim > 64) return s.rows == 32 ? t5::launch<2, 32, 2>(a, pages, grid, stream) : t5::launch<2, 64, 2>(a, pages, grid, stream);
+    if (s.rows == 64) return t5::launch<1, 64, 2>(a, pages, grid, stream);
+    return s.several ? t5::launch<1, 32, 1>(a, pages, grid, stream) : t5::launch<1, 32, 3>(a, pages, grid, stream);
   }
   if (head_dim <= 32) {
     if (s.rows == 16) return launch_mma<32, 1, 1, 4>(a, grid, stream);
