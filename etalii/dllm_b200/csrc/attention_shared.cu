@@ -1459,21 +1459,36 @@ DLLM_EXPORT int dllm_attention_shared_shape(int dtype, int heads, int kv_heads, 
 
 // See the head of the file. out, q [tokens, heads * head_dim] in the cache's type; slots, positions: each token's table row and
 // position; cuts [groups + 1]: the groups' first tokens; shared [groups]: pages from the first on that a group's table rows have
-// in common; the cache entry has `pages` pages.
-DLLM_EXPORT int dllm_attention_shared(void* out, const void* q, int tokens, void* base, long long pages, const int* page_table,
-                                      int max_pages, int page_size, int dtype, int heads, int kv_heads, int head_dim,
-                                      const int* slots, const int* positions, const int* cuts, const int* shared, int groups,
-                                      int max_rows, int max_context, float scale, int window, float* scratch, unsigned* tickets,
-                                      int* status, cudaStream_t stream) {
+// in common; the cache entry has `pages` pages. One structure, `bytes` long, which the caller packs at once.
+struct DllmAttentionShared {
+  void* out;
+  const void* q;
+  void* base;
+  const int *page_table, *slots, *positions, *cuts, *shared;
+  float* scratch;
+  unsigned* tickets;
+  int* status;
+  cudaStream_t stream;
+  long long pages;
+  int tokens, max_pages, page_size, dtype, heads, kv_heads, head_dim, groups, max_rows, max_context, window;
+  float scale;
+};
+DLLM_EXPORT int dllm_attention_shared(const DllmAttentionShared* call, int bytes) {
+  if (bytes != (int)(offsetof(DllmAttentionShared, scale) + sizeof(float))) return DLLM_BAD_ARGUMENT;
+  const DllmAttentionShared& c = *call;
+  const int dtype = c.dtype, heads = c.heads, kv_heads = c.kv_heads, head_dim = c.head_dim, groups = c.groups, max_rows = c.max_rows,
+            max_context = c.max_context;
   if (groups <= 0 || max_rows <= 0) return DLLM_OK;
-  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_context <= 0 || window < 0 || pages <= 0) return DLLM_BAD_ARGUMENT;
-  if (head_dim % 8 || head_dim <= 0 || head_dim > FMA_DIM || page_size != PAGE || kv_heads > 65535 ||
-      ((uintptr_t)out | (uintptr_t)q | (uintptr_t)base) & 15)
+  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_context <= 0 || c.window < 0 || c.pages <= 0) return DLLM_BAD_ARGUMENT;
+  if (head_dim % 8 || head_dim <= 0 || head_dim > FMA_DIM || c.page_size != PAGE || kv_heads > 65535 ||
+      ((uintptr_t)c.out | (uintptr_t)c.q | (uintptr_t)c.base) & 15)
     return DLLM_UNSUPPORTED_SIZE;
   Shape s = shape_of(dtype, heads, kv_heads, head_dim, groups, max_rows, max_context);
   if ((long long)groups * s.tiles > 65535) return DLLM_UNSUPPORTED_SIZE;
-  Args a{out, q, KvLayout{base, page_table, max_pages, page_size, kv_heads, head_dim}, slots, positions, cuts, shared, scratch,
-         tickets, status, heads, window, s.tiles, s.splits, s.cluster, tokens, max_rows, scale};
+  Args a{c.out, c.q, KvLayout{c.base, c.page_table, c.max_pages, c.page_size, kv_heads, head_dim}, c.slots, c.positions, c.cuts,
+         c.shared, c.scratch, c.tickets, c.status, heads, c.window, s.tiles, s.splits, s.cluster, c.tokens, max_rows, c.scale};
+  const long long pages = c.pages;
+  cudaStream_t stream = c.stream;
   dim3 grid(s.splits, kv_heads, groups * s.tiles);
   if (s.kind == FMA) return dtype == DLLM_BF16 ? launch_fma<bf16>(a, grid, stream) : launch_fma<float>(a, grid, stream);
   if (s.kind == TCGEN05) {

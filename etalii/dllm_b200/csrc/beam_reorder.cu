@@ -95,9 +95,16 @@ __global__ void __launch_bounds__(THREADS) reorder_kernel(const Piece* __restric
 }  // namespace
 
 // See the head of the file. `pieces`: the list (device); slots, parents [sequences, beams]; a sequence's length is
-// lengths[sequence * length_stride] + ahead.
-DLLM_EXPORT int dllm_beam_reorder(const void* pieces, int n_pieces, const int* slots, const int* parents, const int* lengths,
-                                  int length_stride, int ahead, int sequences, int beams, int page_size, cudaStream_t stream) {
+// lengths[sequence * length_stride] + ahead. One structure, `bytes` long, which the caller packs at once.
+struct DllmBeamReorder {
+  const void* pieces;
+  const int *slots, *parents, *lengths;
+  cudaStream_t stream;
+  int n_pieces, length_stride, ahead, sequences, beams, page_size;
+};
+DLLM_EXPORT int dllm_beam_reorder(const DllmBeamReorder* call, int bytes) {
+  if (bytes != (int)sizeof(DllmBeamReorder)) return DLLM_BAD_ARGUMENT;
+  const auto [pieces, slots, parents, lengths, stream, n_pieces, length_stride, ahead, sequences, beams, page_size] = *call;
   if (sequences <= 0 || n_pieces <= 0 || beams == 1) return DLLM_OK;
   if (beams <= 0 || page_size <= 0 || length_stride <= 0) return DLLM_BAD_ARGUMENT;
   if (beams > MAX_BEAMS || sequences > 65535) return DLLM_UNSUPPORTED_SIZE;

@@ -5,7 +5,8 @@ from __future__ import annotations
 
 import ctypes
 import functools
-from ctypes import c_double, c_float, c_int, c_longlong, c_void_p
+import struct
+from ctypes import c_char_p, c_double, c_float, c_int, c_longlong, c_void_p
 
 import torch
 
@@ -257,18 +258,17 @@ _prototypes = {
                                   c_float, c_int, c_double, c_double, c_void_p],
     ("sampling", "dllm_seed_rng"): [c_void_p, c_void_p, c_void_p, c_int, c_void_p],
     ("beam_select", "dllm_beam_select_parts"): [c_int, c_int],
-    ("beam_select", "dllm_beam_select"): [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-                                          c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-                                          c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float,
-                                          c_int, c_void_p],
+    ("beam_select", "dllm_beam_select"): [c_char_p, c_int],
     ("attention_shared", "dllm_attention_shared_shape"): [c_int, c_int, c_int, c_int, c_int, c_int, c_int],
-    ("attention_shared", "dllm_attention_shared"): [
-        c_void_p, c_void_p, c_int, c_void_p, c_longlong, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
-        c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
-    ("beam_reorder", "dllm_beam_reorder"): [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
-                                            c_void_p],
+    ("attention_shared", "dllm_attention_shared"): [c_char_p, c_int],
+    ("beam_reorder", "dllm_beam_reorder"): [c_char_p, c_int],
 }
 _functions: dict[tuple[str, str], ctypes._CFuncPtr] = {}
+
+# Calls of a beam search's step, which are short: their arguments are packed at once (the structures of the same names in csrc).
+_BEAM_SELECT = struct.Struct("PqPPPPPPPPPPPPPPPPPiiiiiiiif")
+_BEAM_REORDER = struct.Struct("PPPPPiiiiii")
+_ATTENTION_SHARED = struct.Struct("PPPPPPPPPPPPqiiiiiiiiiiif")
 
 
 launches = 0
@@ -2324,12 +2324,14 @@ def beam_select(parents: torch.Tensor, tokens: torch.Tensor, out: tuple, logits:
     if (stops and stop_ids.dtype is not i32) or (steps is not None and steps.dtype is not i32) or (
             history is not None and (history.dtype is not i32 or history.numel() % places or steps is None)):
         raise KernelError("beam_select: stop_ids, steps and history are int32; history [capacity, sequences, beams] needs steps")
-    _check(_fn("beam_select", "dllm_beam_select")(
-        logits.data_ptr(), vocab, scores.data_ptr(), finished.data_ptr(), finished_at.data_ptr(), done.data_ptr(), produced.data_ptr(), steps.data_ptr() if steps is not None else None, stop_ids.data_ptr() if stops else None, stops,
+    call = _BEAM_SELECT.pack(
+        logits.data_ptr(), vocab, scores.data_ptr(), finished.data_ptr(), finished_at.data_ptr(), done.data_ptr(),
+        produced.data_ptr(), steps.data_ptr() if steps is not None else 0, stop_ids.data_ptr() if stops else 0,
         scores_out.data_ptr(), finished_out.data_ptr(), finished_at_out.data_ptr(), done_out.data_ptr(), parents.data_ptr(),
-        tokens.data_ptr(), history.data_ptr() if history is not None else None,
-        history.numel() // places if history is not None else 0, at, tickets.data_ptr(),
-        sequences, beams_in, beams, vocab, int(min_tokens), float(length_penalty), int(bool(early)), _stream()),
+        tokens.data_ptr(), history.data_ptr() if history is not None else 0, at, tickets.data_ptr(), _stream(), stops,
+        history.numel() // places if history is not None else 0, sequences, beams_in, beams, vocab, min_tokens, bool(early),
+        length_penalty)
+    _check(_fn("beam_select", "dllm_beam_select")(call, _BEAM_SELECT.size),
         "beam_select", lambda: f"{sequences} sequences of {beams_in} beams: at most 65,535 rows")
 
 
@@ -2346,9 +2348,9 @@ def beam_reorder(rows, slots: torch.Tensor, parents: torch.Tensor, lengths: torc
     each, rest = divmod(lengths.numel(), max(1, sequences))
     if slots.numel() != sequences * beams or rest or each not in (1, beams):
         raise KernelError(f"beam_reorder: parents {tuple(parents.shape)}, {slots.numel()} slots, {lengths.numel()} lengths")
-    _check(_fn("beam_reorder", "dllm_beam_reorder")(
-        rows.pieces.data_ptr(), rows.n_pieces, slots.data_ptr(), parents.data_ptr(), lengths.data_ptr(), each, int(ahead),
-        sequences, beams, rows.page_size, _stream()), "beam_reorder", lambda: f"{sequences} sequences: at most 65,535")
+    call = _BEAM_REORDER.pack(rows.pieces.data_ptr(), slots.data_ptr(), parents.data_ptr(), lengths.data_ptr(), _stream(),
+                              rows.n_pieces, each, ahead, sequences, beams, rows.page_size)
+    _check(_fn("beam_reorder", "dllm_beam_reorder")(call, _BEAM_REORDER.size), "beam_reorder", lambda: f"{sequences} sequences: at most 65,535")
 
 
 def decode_advance(tokens: torch.Tensor, tok_pos: torch.Tensor, start: torch.Tensor, chosen: torch.Tensor,
@@ -2448,11 +2450,12 @@ def attention_shared(out: torch.Tensor, q: torch.Tensor, cache, heads: int, scal
         raise KernelError(f"attention_shared: scratch of {scratch.numel()} floats and {tickets.numel()} tickets: {floats} and {words}")
     if max_context > cache.max_pages * cache.page_size:
         raise KernelError(f"attention_shared: contexts of {max_context} in table rows of {cache.max_pages} pages")
-    _check(_fn("attention_shared", "dllm_attention_shared")(
-        out.data_ptr(), q.data_ptr(), tokens, cache.base_ptr, cache.storage.shape[0], cache.page_table.data_ptr(), cache.max_pages, cache.page_size,
-        _code(cache.dtype), heads, cache.kv_heads, cache.head_dim, slots.data_ptr(), positions.data_ptr(), groups.data_ptr(),
-        shared.data_ptr(), count, max_rows, max_context, float(scale), int(window or 0), scratch.data_ptr(), tickets.data_ptr(),
-        _status_word().data_ptr(), _stream()), "attention_shared",
+    call = _ATTENTION_SHARED.pack(
+        out.data_ptr(), q.data_ptr(), cache.base_ptr, cache.page_table.data_ptr(), slots.data_ptr(), positions.data_ptr(),
+        groups.data_ptr(), shared.data_ptr(), scratch.data_ptr(), tickets.data_ptr(), _status_word().data_ptr(), _stream(),
+        cache.storage.shape[0], tokens, cache.max_pages, cache.page_size, _code(cache.dtype), heads, cache.kv_heads, cache.head_dim,
+        count, max_rows, max_context, window or 0, scale)
+    _check(_fn("attention_shared", "dllm_attention_shared")(call, _ATTENTION_SHARED.size), "attention_shared",
         lambda: f"{count} groups of {max_rows} tokens, {heads} heads on {cache.kv_heads} of {cache.head_dim}")
 
 
