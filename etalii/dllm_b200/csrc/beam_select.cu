@@ -13,12 +13,13 @@
 //     beam lives. A sequence that is done keeps its pool, and its places get score -inf.
 //
 // One pass over the logits, in two steps of one launch:
-//   1. A block walks a stretch of a row in tiles of 256 threads x 4 * REG logits, a thread with a maximum and a sum of its own. The
-//      threads form GROUPS groups, at least as many as there are beams; the smallest of the groups' maxima so far is a bound that
-//      at least `beams` logits reach and few do: of logits in any order all groups' maxima lie within the best
-//      GROUPS H(GROUPS), about 54 of 16 groups and 130 of 32. What of a tile reaches the bound goes to a list, which is thinned out by the
-//      latest bound when it fills; at the end each entry counts what is before it. A list that does not hold them all (many
-//      equal logits) is given up for `beams` passes over the stretch.
+//   1. A block walks a stretch of a row in tiles of 256 threads x 4 * REG logits, a thread with a maximum and a sum of its own.
+//      Lane i of all warps is group i; the beams-th largest of the 32 groups' maxima so far is a bound that at least `beams`
+//      logits reach and few do: of logits in any order 4.3, 9.2, 22 for 4, 8, 16 beams (32 H(32) = 130 for 32), so that looking for
+//      them costs little: with the smallest maximum of as many groups as beams or more as the bound, 54 of them for 16
+//      groups, most of the instructions were theirs (32 x 16 beams on 128,256 logits 60.7 us, now 55.4; 1 x 4 on 49,152 9.7, now
+//      8.3). What of a tile reaches the bound goes to a list, which is thinned out by the latest bound when it fills; at the end each entry counts
+//      what is before it. A list that does not hold them all (many equal logits) is given up for `beams` passes over the stretch.
 //   2. The block that finishes last for its sequence (a ticket counter; nobody waits) joins the stretches' sums,
 //      makes the totals and chooses among the stretches' lists the same way; a warp deals out places and pool.
 // Bound by HBM where the rows are many, by the latency of the two steps where they are few. Blocks of a stretch that fits
@@ -64,7 +65,7 @@ struct Shared {
   unsigned long long list[LIST], kept[LIST];
   float list_total[LIST];
   int list_beam[LIST];
-  float group_max[2][THREADS / 32][MAX_BEAMS];
+  float lane_max[2][THREADS / 32][32];
   float warp_m[THREADS / 32], warp_f[THREADS / 32];
   int list_n, seen_n[2], kept_n, last;
   unsigned long long best[2];
@@ -115,21 +116,24 @@ __device__ __forceinline__ float logit_of(unsigned long long word) {
 }
 __device__ __forceinline__ int token_of(unsigned long long word) { return 0x7fffffff - (int)(unsigned)word; }
 
-// The smallest of the groups' maxima of v, which every thread gets. A thread belongs to group threadIdx.x % GROUPS, so that
-// a short stretch has something of every group. `set`: 0 and 1 in turn.
-template <int GROUPS>
-__device__ __forceinline__ float bound_of(float v, Shared& sh, int set) {
+// The rank-th largest of the lanes' maxima of v over the warps, which every thread gets. (A short stretch has something of
+// every lane.) `set`: 0 and 1 in turn.
+__device__ __forceinline__ float bound_of(float v, int rank, Shared& sh, int set) {
   const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int o = 16; o >= GROUPS; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if (lane < GROUPS) sh.group_max[set][threadIdx.x >> 5][lane] = v;
+  sh.lane_max[set][threadIdx.x >> 5][lane] = v;
   __syncthreads();
-  float low = -INFINITY;
+  v = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) low = fmaxf(low, sh.group_max[set][w][lane % GROUPS]);
+  for (int w = 0; w < THREADS / 32; ++w) v = fmaxf(v, sh.lane_max[set][w][lane]);
 #pragma unroll
-  for (int o = GROUPS / 2; o > 0; o >>= 1) low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
-  return low;
+  for (int size = 2; size <= 32; size *= 2)  // sorts the lanes' values, the largest first: lane i holds the i-th
+#pragma unroll
+    for (int o = size / 2; o > 0; o /= 2) {
+      const float other = __shfl_xor_sync(0xffffffffu, v, o);
+      const bool first = (lane & o) == 0, down = (lane & size) == 0;
+      v = first == down ? fmaxf(v, other) : fminf(v, other);
+    }
+  return __shfl_sync(0xffffffffu, v, rank - 1);
 }
 
 // What is done and what its places hold from then on.
@@ -149,7 +153,7 @@ __device__ __forceinline__ void leave_as_is(const Args& a, int b, int* history) 
   if (threadIdx.x == 0) a.done_out[b] = 1;
 }
 
-template <int REG, int GROUPS>
+template <int REG>
 __global__ void __launch_bounds__(THREADS, 4) select_kernel(const Args a) {
   __shared__ Shared sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -225,7 +229,7 @@ __global__ void __launch_bounds__(THREADS, 4) select_kernel(const Args a) {
 #pragma unroll
       for (int e = 0; e < 4 * REG; ++e) top = fmaxf(top, v[e]);
       // The bound goes by what may be chosen: what a thread has in a tile beside a stop token does not take part in it (any
-      // logits of at least `beams` groups make a bound).
+      // logits of at least `beams` lanes make a bound).
       bool beside = false;
       for (int s = 0; s < n_stops; ++s) {
         const int at = ((sh.stops[s] - first) >> 2) - tile * REG * THREADS;
@@ -234,7 +238,7 @@ __global__ void __launch_bounds__(THREADS, 4) select_kernel(const Args a) {
       if (!beside) keep = fmaxf(keep, top);
       if ((tile & (tile - 1)) == 0) {  // a new bound with the first, the second, the third, the fifth, the ninth tile ..: no barrier between
         if (tid == 0) sh.seen_n[updates & 1] = sh.list_n;  // (of the tiles before; a late entry of the last one may be missing)
-        low = bound_of<GROUPS>(keep, sh, updates & 1);
+        low = bound_of(keep, beams, sh, updates & 1);
         floor_ = fmaxf(low, -FLT_MAX);  // (-inf is no candidate)
         if (sh.seen_n[updates & 1] > LIST / 2) {  // thin out the list
           __syncthreads();
@@ -299,7 +303,7 @@ __global__ void __launch_bounds__(THREADS, 4) select_kernel(const Args a) {
       const unsigned long long* from = sh.list;
       int kept = n;
       if (tiles > 1) {
-        low = bound_of<GROUPS>(keep, sh, updates & 1);
+        low = bound_of(keep, beams, sh, updates & 1);
         const unsigned long long least = word_of(fmaxf(low, -FLT_MAX), 0x7fffffff);
         for (int c = tid; c < n; c += THREADS)
           if (sh.list[c] >= least) sh.kept[atomicAdd(&sh.kept_n, 1)] = sh.list[c];
@@ -438,7 +442,7 @@ __global__ void __launch_bounds__(THREADS, 4) select_kernel(const Args a) {
     sh.stop[tid] = Candidate{total, stop_logit, stop_beam, stop_token};
     sh.stop_total[tid] = total;
   }
-  const float low = bound_of<GROUPS>(top, sh, 0), floor_ = fmaxf(low, -FLT_MAX);
+  const float low = bound_of(top, beams, sh, 0), floor_ = fmaxf(low, -FLT_MAX);
   auto offer = [&](const Candidate& one) {
     const int to = atomicAdd(&sh.list_n, 1);
     if (to < LIST) {
@@ -583,17 +587,21 @@ __global__ void __launch_bounds__(THREADS, 4) select_kernel(const Args a) {
     a.done_out[b] = (worst > -INFINITY && (a.early || worst >= best / length)) || best == -INFINITY ? 1 : 0;
 }
 
-// Stretches a row is cut into: as many as fill the device, of 2,048 logits at least.
+// Stretches a row is cut into: as many as fill the device, one more where a quarter of it would stay idle, of 2,048 logits at
+// least. (us with that many and with one more, 128,256 logits: 304 rows 55.8 and 39.3, 352 rows 58.1 and 52.7, 448 rows 59.1 and
+// 57.1, 496 rows 59.6 and 60.8; 200 rows, two or three, 37.8 and 32.4; of 49,152: 200 rows 21.2 and 18.6, 304 rows 30.5 and
+// 23.6, 400 rows 32.3 and 32.3; 40 rows, 14 or 15, 15.4 and 18.3.)
 int parts_for(int rows, int vocab) {
-  const int most = (vocab - 1) / 2048 + 1, wanted = PLACES / (rows < PLACES ? rows : PLACES);
+  const int most = (vocab - 1) / 2048 + 1;
+  int wanted = PLACES / (rows < PLACES ? rows : PLACES);
+  if (4ll * wanted * rows <= 3 * PLACES) ++wanted;
   return wanted < most ? wanted : most;
 }
 
 template <int REG>
 int launch(const Args& a, int sequences, int parts, cudaStream_t stream) {
   dim3 grid(parts, sequences * a.beams_in), block(THREADS);
-  return a.beams <= 16 ? dllm_launch_pdl(select_kernel<REG, 16>, grid, block, 0, stream, a)
-                       : dllm_launch_pdl(select_kernel<REG, 32>, grid, block, 0, stream, a);
+  return dllm_launch_pdl(select_kernel<REG>, grid, block, 0, stream, a);
 }
 }  // namespace
 
