@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(THREADS, 4) select_kernel(const Args a) {
     __threadfence();  // (what the block has written, which the barrier has shown to this thread, before the ticket)
     sh.last = atomicAdd(&a.tickets[b], 1u) == (unsigned)(a.beams_in * parts - 1);
     __threadfence();
-    sh.list_n = 0;
+    sh.list_n = sh.kept_n = 0;
   }
   __syncthreads();
   if (!sh.last) return;
@@ -372,10 +372,12 @@ __global__ void __launch_bounds__(THREADS, 4) select_kernel(const Args a) {
     const int list = list_of(c);
     return __ldcg(reinterpret_cast<const float2*>(all + (size_t)list * entry + 2 + 2 * (c - list * beams)));
   };
-  constexpr int HELD = 4;  // what a thread looks at first stays with it
+  constexpr int HELD = 4;  // entries stay with a thread, where they are not more than that
+  const bool by_lists = n_entries > HELD * THREADS;
+  const int n_held = by_lists ? 0 : n_entries;
   float2 held[HELD];
 #pragma unroll
-  for (int u = 0; u < HELD; ++u) held[u] = tid + u * THREADS < n_entries ? pair_at(tid + u * THREADS) : make_float2(-INFINITY, 0.f);
+  for (int u = 0; u < HELD; ++u) held[u] = tid + u * THREADS < n_held ? pair_at(tid + u * THREADS) : make_float2(-INFINITY, 0.f);
   const bool may_end = step >= a.min_tokens;
   const int n_stop = may_end ? a.beams_in * n_stops : 0;  // (at most THREADS)
   int stop_beam = 0, stop_token = -1;
@@ -433,10 +435,11 @@ __global__ void __launch_bounds__(THREADS, 4) select_kernel(const Args a) {
 #pragma unroll
   for (int u = 0; u < HELD; ++u) {
     const int c = tid + u * THREADS;
-    totals[u] = c < n_entries ? total_of(held[u].x, beam_of(c)) : -INFINITY;
+    totals[u] = c < n_held ? total_of(held[u].x, beam_of(c)) : -INFINITY;
     top = fmaxf(top, totals[u]);
   }
-  for (int c = tid + HELD * THREADS; c < n_entries; c += THREADS) top = fmaxf(top, candidate_at(c).total);
+  if (by_lists)  // (the lists' firsts alone)
+    for (int list = tid; list < n_lists; list += THREADS) top = fmaxf(top, candidate_at(list * beams).total);
   if (tid < n_stop) {
     const float total = stop_token >= 0 && stop_token < vocab ? total_of(stop_logit, stop_beam) : -INFINITY;
     sh.stop[tid] = Candidate{total, stop_logit, stop_beam, stop_token};
@@ -454,9 +457,16 @@ __global__ void __launch_bounds__(THREADS, 4) select_kernel(const Args a) {
 #pragma unroll
   for (int u = 0; u < HELD; ++u)
     if (totals[u] >= floor_) offer(Candidate{totals[u], held[u].x, beam_of(tid + u * THREADS), __float_as_int(held[u].y)});
-  for (int c = tid + HELD * THREADS; c < n_entries; c += THREADS) {
-    const Candidate one = candidate_at(c);
-    if (one.total >= floor_) offer(one);
+  if (by_lists) {  // (at most LIST of them: parts_for.) A list is in order: one whose first does not reach the bound has nothing that does
+    for (int list = tid; list < n_lists; list += THREADS)
+      if (candidate_at(list * beams).total >= floor_) sh.kept[atomicAdd(&sh.kept_n, 1)] = list;
+    __syncthreads();
+    const int n = sh.kept_n * beams;
+    for (int c = tid; c < n; c += THREADS) {
+      const int list = list_of(c);
+      const Candidate one = candidate_at((int)sh.kept[list] * beams + c - list * beams);
+      if (one.total >= floor_) offer(one);
+    }
   }
   __syncthreads();
   auto listed = [&](int c) {
@@ -587,15 +597,24 @@ __global__ void __launch_bounds__(THREADS, 4) select_kernel(const Args a) {
     a.done_out[b] = (worst > -INFINITY && (a.early || worst >= best / length)) || best == -INFINITY ? 1 : 0;
 }
 
-// Stretches a row is cut into: as many as fill the device, one more where a quarter of it would stay idle, of 2,048 logits at
-// least. (us with that many and with one more, 128,256 logits: 304 rows 55.8 and 39.3, 352 rows 58.1 and 52.7, 448 rows 59.1 and
-// 57.1, 496 rows 59.6 and 60.8; 200 rows, two or three, 37.8 and 32.4; of 49,152: 200 rows 21.2 and 18.6, 304 rows 30.5 and
-// 23.6, 400 rows 32.3 and 32.3; 40 rows, 14 or 15, 15.4 and 18.3.)
+// Stretches a row is cut into: as many as fill the device, one more where a quarter of it would stay idle, as many more as save a
+// tile where a tenth of them have to wait; of 2,048 logits at least, and not more than a warp joins at once while they are a tile
+// at most. (us on 128,256 logits: 304 rows, one or two stretches, 45.7 and 34.0, 352 rows 58.1 and 52.7, 496 rows 50.1 and 53.0; 160
+// rows, three or four, 26.1 and 22.4; 80 rows, seven or eight, 19.4 and 17.2; 64 rows, nine or sixteen, 17.5 and 17.4; 16 rows, 37
+// or 16 to 32, 12.2 and 10.9; 4 rows, 63 or 16 to 32, 9.5 and 9.0. Of 49,152: 304 rows 26.3 and 21.2, 200 rows, two or three, 18.5 and 16.0,
+// 40 rows, 14 or 15, 11.9 and 13.7.)
 int parts_for(int rows, int vocab) {
-  const int most = (vocab - 1) / 2048 + 1;
+  constexpr int TILE = THREADS * 4 * 8;
   int wanted = PLACES / (rows < PLACES ? rows : PLACES);
   if (4ll * wanted * rows <= 3 * PLACES) ++wanted;
-  return wanted < most ? wanted : most;
+  const int tiles = (vocab - 1) / (wanted * TILE) + 1;
+  if (tiles > 1) {
+    const int more = (vocab - 1) / ((tiles - 1) * TILE) + 1;
+    if (10ll * more * rows <= 11 * PLACES) wanted = more;
+  }
+  const int each = (vocab - 1) / TILE + 1, most = (vocab - 1) / 2048 + 1, enough = each > 32 ? each : 32;
+  if (wanted > most) wanted = most;
+  return wanted < enough ? wanted : enough;
 }
 
 template <int REG>

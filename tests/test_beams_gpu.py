@@ -117,6 +117,22 @@ def test_choice(n, rows, beams, vocab, stops):
     case.check(case.run(penalty=0.7, early=True), penalty=0.7, early=True)
 
 
+@pytest.mark.parametrize("n,rows,beams,vocab", [(1, 16, 16, 33001), (1, 32, 32, 16003), (2, 9, 9, 30011), (1, 16, 32, 9001),
+                                                (5, 16, 16, 12289)])
+@pytest.mark.parametrize("what", ["any", "one row", "equal rows", "few"])
+def test_choice_among_many_lists(n, rows, beams, vocab, what):
+    """More candidates in the stretches' lists than a block holds at a time: it goes by the lists' first."""
+    case = Choice(n, rows, beams, vocab, seed=vocab + beams, stops=(3, vocab - 1))
+    if what == "one row":
+        case.scores[:, 1:] = -math.inf  # (one beam lives)
+    elif what == "equal rows":
+        case.logits[:] = case.logits[0].round()  # (totals tie in every row and list)
+        case.scores[:] = -1.0
+    elif what == "few":
+        case.logits[:, 7:] = -math.inf  # (fewer candidates than lists)
+    case.check(case.run(penalty=0.7), penalty=0.7)
+
+
 @pytest.mark.parametrize("penalty,early", [(0.0, False), (1.0, False), (1.3, True)])
 @pytest.mark.parametrize("produced,min_tokens", [(0, 0), (3, 5), (5, 5), (900, 5)])
 def test_choice_of_lengths_and_ends(penalty, early, produced, min_tokens):
