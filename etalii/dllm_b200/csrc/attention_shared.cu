@@ -1402,15 +1402,16 @@ Shape shape_of(int dtype, int heads, int kv_heads, int head_dim, int groups, int
   else s.rows = query_rows <= 32 ? 32 : 64;
   s.tiles = (query_rows + s.rows - 1) / s.rows;
   // Blocks of a tile and kv head: as many as fill the device, but not more than there can be pages, in the largest clusters that
-  // do not cost more than a fifth of them; where there are at most 64 pages one cluster, which needs no scratch and no second
-  // round. (Clusters of 1 to 8 blocks that are resident at a time: a cluster lies within a part of the device, and what is left over of
+  // do not cost more than a fifth of them; where there are at most 64 pages one cluster, which needs no scratch and no second round (by
+  // multiply-adds, where a page costs more, at most 16: 9 heads on 3 of 64, 2 x 5 beams on 700 positions, one cluster of 8 18.0 us,
+  // three of 7 14.9; 4 x 4 on 2,000 28.5 and 20.8). (Clusters of 1 to 8 blocks that are resident at a time: a cluster lies within a part of the device, and what is left over of
   // a part stays idle. The last few that would fit start late behind another kernel's blocks: float32, clusters of 8, 31 of them 28.4 us, 33
   // 36.2.) Eight new tokens a prompt, 32 heads on 8 of 128, us with one cluster of 8, 4 of 4, 9 of 2 and 18 of 1: 2,000 positions
   // 13.4, 17.2, 20.7, 24.1; 80,000: -, 62.6, 65.9, 70.1. Sizes that are no powers of two: three prompts of 20,000 positions 46.8
   // with three clusters of 2, 44.0 with one of 5; five of 10,000 43.8 with three of 1, 38.7 with one of 3; 2 x 8 beams on 2,000 16.1 with
   // one of 4, 13.6 with one of 6.
   static const int RESIDENT[2][MAX_CLUSTER] = {{148, 74, 44, 33, 25, 22, 15, 15}, {296, 148, 90, 70, 54, 44, 36, 31}};
-  const long long pairs = (long long)groups * s.tiles * kv_heads, most = pages + max_rows;
+  const long long pairs = (long long)groups * s.tiles * kv_heads, most = pages + (s.kind == FMA ? 2 : 1) * max_rows;
   // (Two blocks for heads of 64 and 32 rows where there are more pairs than multiprocessors: 32 heads on 32, 8 x 4 beams on 60, 1,000,
   // 2,000 and 4,000 positions 20.0, 30.7, 37.7, 53.5 us with one, 13.6, 25.1, 36.4, 56.0 with two; 16 x 4 on 1,000 and 4,000 57.6, 104 and
   // 43.8, 91.7.)
@@ -1420,7 +1421,7 @@ Shape shape_of(int dtype, int heads, int kv_heads, int head_dim, int groups, int
   for (int c = 1; c <= MAX_CLUSTER; ++c) {
     long long n = RESIDENT[s.several][c - 1] / pairs;
     if (n > MAX_CLUSTERS) n = MAX_CLUSTERS;
-    if (pages <= 64 && n > 1) n = c > 1 ? 1 : 0;
+    if ((s.kind == FMA ? most <= 16 : pages <= 64) && n > 1) n = c > 1 ? 1 : 0;
     if (n * c > most) n = most / c;
     blocks[c - 1] = n * c;
     if (n * c > best) best = n * c;
