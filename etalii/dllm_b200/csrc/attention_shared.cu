@@ -721,8 +721,10 @@ int launch_clusters(Kernel kernel, dim3 grid, int threads, size_t smem, int clus
 // their pages, P^T written as [key][row]). A product then reads 128 x 16 values of a page and ROWS x 16 others; with the query
 // rows as the 128-row operand (padded) it would read those 128 x 16 for every 64 keys: 768 cycles of shared memory a page
 // for heads of 128 instead of 320.
-//   softmax warps  two groups that take the steps in turn, each with scores, P and outputs of its own: a thread has a key
-//                  and 32 query rows. A row's maximum over the step goes through redux and shared memory; where it grew the
+//   softmax warps  GROUPS groups that take the steps in turn, each with scores, P and outputs of its own: a thread has a key
+//                  and 32 query rows. (Three groups for heads of 64, two above, one where there are 64 rows: a second one left 96
+//                  registers a thread, 200 bytes of them spilled; 9 heads on 3 of 64, 16 new tokens on 1,000 positions 10.9 us, 9.0 with
+//                  one; 32 on 8 of 128 on 16,000, eight prompts, 117.8 and 109.3. One, too, for two blocks of a multiprocessor.) A row's maximum over the step goes through redux and shared memory; where it grew the
 //                  group's outputs are scaled in tensor memory (32 columns). Every step uses the running maximum itself, so
 //                  that the largest weight is 1 and not rounded.
 //   three more     one looks pages up, 32 at a time, and issues their TMA loads; one issues the scores' products, one the
@@ -736,10 +738,10 @@ constexpr int KEYS = 2 * PAGE;
 constexpr int P_BYTES = KEYS * 128;  // [key][64 rows]
 
 template <int BOXES, int ROWS, int GROUPS> struct Shape {
-  static constexpr int BLOCKS = GROUPS == 1 ? 2 : 1;            // of a multiprocessor
+  static constexpr int BLOCKS = GROUPS == 1 && ROWS == 32 ? 2 : 1;  // of a multiprocessor
   static constexpr int HALVES = ROWS / 32;                      // warps that share a step's keys, 32 rows each
   static constexpr int GROUP = 4 * HALVES, SOFT_WARPS = GROUPS * GROUP, THREADS = (SOFT_WARPS + 3) * 32;
-  static constexpr int K_STAGES = BOXES == 2 || GROUPS == 1 ? 2 : 4, V_STAGES = GROUPS == 1 ? 2 : BOXES == 2 ? 3 : 5;
+  static constexpr int K_STAGES = BOXES == 2 || BLOCKS == 2 ? 2 : 4, V_STAGES = BLOCKS == 2 ? 2 : BOXES == 2 ? 3 : 5;
   static constexpr int Q_BYTES = BOXES * ROWS * 128, KV_BYTES = BOXES * KEYS * 128;
   static constexpr unsigned COLUMNS = 2 * GROUPS * ROWS > 128 ? 256 : 2 * GROUPS * ROWS > 64 ? 128 : 64;  // of tensor memory: scores and outputs
   static constexpr int SMEM = Q_BYTES + GROUPS * P_BYTES + (K_STAGES + V_STAGES) * KV_BYTES + 1024;
@@ -1499,8 +1501,8 @@ DLLM_EXPORT int dllm_attention_shared(const DllmAttentionShared* call, int bytes
   if (s.kind == FMA) return dtype == DLLM_BF16 ? launch_fma<bf16>(a, grid, stream) : launch_fma<float>(a, grid, stream);
   if (s.kind == TCGEN05) {
     if (pages * 2 * kv_heads * PAGE > 0x7fffffffll) return DLLM_UNSUPPORTED_SIZE;  // (a TMA coordinate is an int)
-    if (head_dim > 64) return s.rows == 32 ? t5::launch<2, 32, 2>(a, pages, grid, stream) : t5::launch<2, 64, 2>(a, pages, grid, stream);
-    if (s.rows == 64) return t5::launch<1, 64, 2>(a, pages, grid, stream);
+    if (head_dim > 64) return s.rows == 32 ? t5::launch<2, 32, 2>(a, pages, grid, stream) : t5::launch<2, 64, 1>(a, pages, grid, stream);
+    if (s.rows == 64) return t5::launch<1, 64, 1>(a, pages, grid, stream);
     return s.several ? t5::launch<1, 32, 1>(a, pages, grid, stream) : t5::launch<1, 32, 3>(a, pages, grid, stream);
   }
   if (head_dim <= 32) {
