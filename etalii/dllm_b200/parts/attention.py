@@ -43,9 +43,10 @@ def reads_shared_pages(batch, cache) -> bool:
     whatever the contexts are, where the kernels that read every token's pages cost 3 to 10 µs and then grow with them. Beams: from
     so many bytes of keys and values on, counted for every beam (heads up to 64, above; and 1 MB for every prompt and kv head: their
     blocks take turns). Short chunks: from 768 positions on. Measured, µs, shared and not: 8 x 8 beams, 9 heads on 3 of 64,
-    1,000 positions 12.3 and 8.8, 4,000 16.2 and 20.3; 32 heads on 8 of 128, 500 positions 16.4 and 28.1, 4,000 32.7 and 102.5; 1 x 4, 2,000
-    positions 13.0 and 9.2, 4,000 15.0 and 15.3; float32, 9 heads on 3 of 64, 8 x 8 beams on 250 positions 21.1 and 17.8, on 2,000 49.9 and
-    106.6; eight new tokens on 250, 1,000 and 16,000 positions, 32 heads on 8 of 128, 10.0 and 9.3, 10.2 and 16.3, 23.4 and 166.9."""
+    1,000 positions 11.8 and 8.7, 4,000 15.0 and 20.4; 32 heads on 8 of 128, 500 positions 15.9 and 28.0, 4,000 32.4 and 102.5; 1 x 4, 2,000
+    positions 13.1 and 9.6, 4,000 15.2 and 15.6; 32 heads on 32 of 64, 8 x 4 on 500 19.5 and 20.2, on 1,000 26.6 and 31.2; float32, 9 heads
+    on 3 of 64, 8 x 8 beams on 250 positions 20.8 and 17.8, on 2,000 41.3 and 106.8; eight new tokens on 250, 1,000 and 16,000 positions, 32
+    heads on 8 of 128, 9.3 and 9.3, 9.4 and 16.3, 23.0 and 167.4."""
     shared = getattr(batch, "shared", None)
     if shared is None or not ops.attention_shared_supported(cache):
         return False
