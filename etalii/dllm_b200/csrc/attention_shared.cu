@@ -724,11 +724,12 @@ int launch_clusters(Kernel kernel, dim3 grid, int threads, size_t smem, int clus
 // rows as the 128-row operand (padded) it would read those 128 x 16 for every 64 keys: 768 cycles of shared memory a page
 // for heads of 128 instead of 320.
 //   softmax warps  GROUPS groups that take the steps in turn, each with scores, P and outputs of its own: a thread has a key
-//                  and 32 query rows. (Three groups for heads of 64, two above, one where there are 64 rows: a second one left 96
-//                  registers a thread, 200 bytes of them spilled; 9 heads on 3 of 64, 16 new tokens on 1,000 positions 10.9 us, 9.0 with
-//                  one; 32 on 8 of 128 on 16,000, eight prompts, 117.8 and 109.3. One, too, for two blocks of a multiprocessor.) A row's maximum over the step goes through redux and shared memory; where it grew the
+//                  and 32 query rows. A row's maximum over the step goes through redux and shared memory; where it grew the
 //                  group's outputs are scaled in tensor memory (32 columns). Every step uses the running maximum itself, so
-//                  that the largest weight is 1 and not rounded.
+//                  that the largest weight is 1 and not rounded. Three groups for heads of 64, two above, one for two blocks of a
+//                  multiprocessor, and one where there are 64 rows: a second left 96 registers a thread and 200 bytes
+//                  spilled (9 heads on 3 of 64, 16 new tokens on 1,000 positions 10.9 us, 9.0 with one; 32 on 8 of 128, eight
+//                  prompts of 16,000, 117.8 and 109.3; 8 x 16 beams on 2,000 37.9 and 39.3).
 //   three more     one looks pages up, 32 at a time, and issues their TMA loads; one issues the scores' products, one the
 //                  outputs'.
 // Pages that some row sees in part are looked at: a value that is not finite is kept out of the product; such a step is added
@@ -1412,14 +1413,16 @@ Shape shape_of(int dtype, int heads, int kv_heads, int head_dim, int groups, int
   else s.rows = query_rows <= 32 ? 32 : 64;
   s.tiles = (query_rows + s.rows - 1) / s.rows;
   // Blocks of a tile and kv head: as many as fill the device, but not more than there can be pages, in the largest clusters that
-  // do not cost more than a fifth of them; where there are at most 64 pages one cluster, which needs no scratch and no second round (by
-  // multiply-adds, where a page costs more, at most 16: 9 heads on 3 of 64, 2 x 5 beams on 700 positions, one cluster of 8 18.0 us,
-  // three of 7 14.9; 4 x 4 on 2,000 28.5 and 20.8). (Clusters of 1 to 8 blocks that are resident at a time: a cluster lies within a part of the device, and what is left over of
-  // a part stays idle. The last few that would fit start late behind another kernel's blocks: float32, clusters of 8, 31 of them 28.4 us, 33
-  // 36.2.) Eight new tokens a prompt, 32 heads on 8 of 128, us with one cluster of 8, 4 of 4, 9 of 2 and 18 of 1: 2,000 positions
-  // 13.4, 17.2, 20.7, 24.1; 80,000: -, 62.6, 65.9, 70.1. Sizes that are no powers of two: three prompts of 20,000 positions 46.8
-  // with three clusters of 2, 44.0 with one of 5; five of 10,000 43.8 with three of 1, 38.7 with one of 3; 2 x 8 beams on 2,000 16.1 with
+  // do not cost more than a fifth of them; where there are at most 64 pages one cluster, which needs no scratch and no second
+  // round (by multiply-adds, where a page costs more, at most 16: 9 heads on 3 of 64, 2 x 5 beams on 700 positions, one cluster
+  // of 8 18.0 us, three of 7 14.9; 4 x 4 on 2,000 28.5 and 20.8).
+  // Eight new tokens a prompt, 32 heads on 8 of 128, us with one cluster of 8, 4 of 4, 9 of 2 and 18 of 1: 2,000 positions 13.4, 17.2,
+  // 20.7, 24.1; 80,000: -, 62.6, 65.9, 70.1. Sizes that are no powers of two: three prompts of 20,000 positions 46.8 with three
+  // clusters of 2, 44.0 with one of 5; five of 10,000 43.8 with three of 1, 38.7 with one of 3; 2 x 8 beams on 2,000 16.1 with
   // one of 4, 13.6 with one of 6.
+  // RESIDENT: clusters of 1 to 8 blocks that start together, one and two blocks a multiprocessor. A cluster lies within a part of
+  // the device, and what is left over of a part stays idle; the last few that would fit start late behind another kernel's blocks
+  // (float32, two blocks, clusters of 8: 31 of them 28.4 us, 33 36.2).
   static const int RESIDENT[2][MAX_CLUSTER] = {{148, 74, 44, 33, 25, 22, 15, 15}, {296, 148, 90, 70, 54, 44, 36, 31}};
   const long long pairs = (long long)groups * s.tiles * kv_heads, most = pages + (s.kind == FMA ? 2 : 1) * max_rows;
   // (Two blocks for heads of 64 and 32 rows where there are more pairs than multiprocessors: 32 heads on 32, 8 x 4 beams on 60, 1,000,
