@@ -333,9 +333,9 @@ __device__ __forceinline__ void finish(Plan& p, const Args& a, const float* x, i
   __syncthreads();
   if (threadIdx.x == 0) {
     unsigned* ticket = a.tickets + pair * size + rank;
-    __threadfence();  // (what the block has written, which the barrier has shown to this thread, before the ticket)
-    p.last = atomicAdd(ticket, 1u) == (unsigned)(clusters - 1);
-    __threadfence();
+    unsigned before;  // (acquire and release: what the block has written, which the barrier has shown to this thread, and the others)
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(ticket) : "memory");
+    p.last = before == (unsigned)(clusters - 1);
     if (p.last) *ticket = 0u;
   }
   __syncthreads();

@@ -22,8 +22,8 @@
 //      what is before it. A list that does not hold them all (many equal logits) is given up for `beams` passes over the stretch.
 //   2. The block that finishes last for its sequence (a ticket counter; nobody waits) joins the stretches' sums,
 //      makes the totals and chooses among the stretches' lists the same way; a warp deals out places and pool.
-// Bound by HBM where the rows are many, by the latency of the two steps where they are few: 1 x 4 beams of 49,152 logits 8.1 us (2.5 to the
-// stretch's best, 1 for the ticket, 4.3 for the join), 8 x 8 of 128,256 17.6, 32 x 16 55.1 (230 MB of living rows, 4.2 TB/s; 6.3 while all
+// Bound by HBM where the rows are many, by the latency of the two steps where they are few: 1 x 4 beams of 49,152 logits 7.9 us (2.5 to the
+// stretch's best, 1 for the ticket, 4 for the join), 8 x 8 of 128,256 17.3, 32 x 16 54.6 (230 MB of living rows, 4.2 TB/s; 6.3 while all
 // multiprocessors have as many blocks, but 448 living rows are four for some and three for others). Blocks of a stretch that fits
 // their registers (4,096 of them for 512 rows of 128,256 instead of 512) spent most of their time on what a block costs. The next tile
 // by bulk copies into shared memory while this one is worked on changed nothing (8 x 8 18.0 us where it was 18.7, 32 x 16 57.1 where it was 55.4).
@@ -355,9 +355,11 @@ __global__ void __launch_bounds__(THREADS, 4) select_kernel(const Args a) {
   // ---- who is last?
   __syncthreads();
   if (tid == 0) {
-    __threadfence();  // (what the block has written, which the barrier has shown to this thread, before the ticket)
-    sh.last = atomicAdd(&a.tickets[b], 1u) == (unsigned)(a.beams_in * parts - 1);
-    __threadfence();
+    // Acquire and release in one: what the block has written, which the barrier has shown to this thread, and what the others have
+    // (fences before and after the ticket 8.2 us, 7.9: 1 x 4 beams of 49,152 logits).
+    unsigned before;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(a.tickets + b) : "memory");
+    sh.last = before == (unsigned)(a.beams_in * parts - 1);
     sh.list_n = sh.kept_n = 0;
   }
   __syncthreads();
