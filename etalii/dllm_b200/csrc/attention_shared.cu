@@ -10,7 +10,7 @@
 // a list of pages: those in common, then the tokens' own, each once for the tokens that have it. The list is cut into
 // `splits` stretches of equal length, a block each, so that the device is filled whatever the contexts are; running maximum
 // and sum are kept in float32. Up to eight blocks form a cluster and add their results up through distributed shared memory; where there
-// are more clusters, theirs go to scratch, and of the blocks that have written the same pieces of it the last (a ticket;
+// are more clusters, theirs go to scratch, and of the blocks that have written the same rows of it the last (a ticket;
 // nobody waits) joins them in order.
 //
 // bfloat16, head sizes that are multiples of 16: from 64 to 128 on the 5th-generation tensor cores (namespace t5), below
@@ -238,11 +238,6 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n"
                "barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
-// The same without an order of memory: for those that wait until others have read what is theirs.
-__device__ __forceinline__ void cluster_wait_for_readers() {
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n"
-               "barrier.cluster.wait.aligned;\n" ::: "memory");
-}
 __device__ __forceinline__ unsigned remote_addr(const void* local, unsigned rank) {
   unsigned addr = (unsigned)__cvta_generic_to_shared(local), remote;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
@@ -277,17 +272,20 @@ __device__ __forceinline__ void write_out(const Plan& p, const Args& a, int r, i
 }
 
 // Every block has its result in shared memory: x[row * ld ..] sums, ml[row] (maximum, sum); a block without pages has (-inf, 0)
-// there and anything in x. The blocks of the cluster take the rows' pieces in turn. All threads call.
+// there and anything in x. The blocks of the cluster share the rows out, whole rows, so that whoever joins sums of a row also has
+// written its maximum and sum (pieces dealt out in turn cross rows wherever a row's are no divisor of a block's threads). All
+// threads call.
 template <typename T, int ROWS>
 __device__ __forceinline__ void finish(Plan& p, const Args& a, const float* x, int ld, const float2* ml) {
   const int hd = a.cache.head_dim, fours = hd / 4, clusters = a.splits / a.cluster;
   const unsigned size = a.cluster, rank = blockIdx.x % size;
+  const int from = p.rows * rank / size * fours, to = p.rows * (rank + 1) / size * fours;  // this block's pieces
   const size_t pair = (size_t)blockIdx.z * gridDim.y + blockIdx.y;
   float* parts = a.scratch;
   float* part_ml = a.scratch + (size_t)gridDim.z * gridDim.y * clusters * ROWS * hd;
   if (size > 1) cluster_sync();
   else __syncthreads();
-  for (int i = rank * blockDim.x + threadIdx.x; i < p.rows * fours; i += size * blockDim.x) {
+  for (int i = from + threadIdx.x; i < to; i += blockDim.x) {
     const int r = i / fours, d = (i % fours) * 4;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     float top = -INFINITY, total = 0.f;
@@ -327,9 +325,11 @@ __device__ __forceinline__ void finish(Plan& p, const Args& a, const float* x, i
       if (d == 0) *reinterpret_cast<float2*>(part_ml + at * 2) = make_float2(top, total);
     }
   }
-  if (size > 1) cluster_wait_for_readers();  // nobody leaves while others read its result
+  // Nobody leaves while others read its result. (With the order of memory: a value that a thread has asked for and does not use is
+  // read too.)
+  if (size > 1) cluster_sync();
   if (clusters == 1) return;
-  // Blocks of one rank have written the same pieces, one cluster's part each: the last of them joins these, in order.
+  // Blocks of one rank have written the same rows, one cluster's part each: the last of them joins these, in order.
   __syncthreads();
   if (threadIdx.x == 0) {
     unsigned* ticket = a.tickets + pair * size + rank;
@@ -340,7 +340,7 @@ __device__ __forceinline__ void finish(Plan& p, const Args& a, const float* x, i
   }
   __syncthreads();
   if (!p.last) return;
-  for (int i = rank * blockDim.x + threadIdx.x; i < p.rows * fours; i += size * blockDim.x) {
+  for (int i = from + threadIdx.x; i < to; i += blockDim.x) {
     const int r = i / fours, d = (i % fours) * 4;
     float top = -INFINITY, total = 0.f;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);

@@ -509,6 +509,35 @@ def test_attention_twice_gives_the_same_bits(dtype, dim):
         assert np.array_equal(first, pages.run(repeat=3))
 
 
+@pytest.mark.parametrize("dtype,dim", [(torch.float32, 24), (torch.float32, 72), (torch.float32, 80), (torch.float32, 136), (torch.bfloat16, 48),
+                                       (torch.bfloat16, 80), (torch.bfloat16, 96), (torch.bfloat16, 112), (torch.bfloat16, 136)])
+def test_attention_of_several_clusters_whose_rows_do_not_divide_a_block(dtype, dim):
+    """Contexts that several clusters share, head sizes whose rows' pieces do not end where a block's threads do, other values in the
+    same scratch from call to call: each output row takes its maximum and sum from its own call."""
+    from etalii.dllm_b200.cache.paged import KvView
+
+    o = ops()
+    both = [Pages("chunk", [(0, list(range(9000, 9008)))] * n, 8, 1, dim, dtype, seed=n, values=v) for n, v in ((1, 1.0), (2, 4.0))]
+    sizes = [o.attention_shared_scratch(KvView(p.storage.to(DEV), p.table.to(DEV), 64, 1, dim, None), 8, len(p.cuts) - 1, 8, 9008) for p in both]
+    assert all(floats > 0 and words > 0 for floats, words in sizes)  # (several clusters)
+    scratch = torch.full((max(floats for floats, _ in sizes),), math.nan, device=DEV)
+    tickets = torch.zeros(max(words for _, words in sizes), dtype=torch.int32, device=DEV)
+    calls = []
+    for p in both:
+        view = KvView(p.storage.to(DEV), p.table.to(DEV), 64, 1, dim, None)
+        q, want = p.q.to(DEV), p.want()
+        calls.append((p, view, q, want, [_i32(x) for x in (p.slots, p.positions, p.cuts, p.shared)]))
+    results = []
+    for _ in range(3):
+        for p, view, q, want, rest in calls:
+            out = torch.full_like(q, 7.0)
+            o.attention_shared(out, q, view, 8, p.scale, 0, *rest, 8, 9008, scratch, tickets)
+            results.append(out.float().cpu().numpy())
+            assert np.abs(results[-1] - want).max() <= p.tolerance()
+    o.raise_if_failed()
+    assert all(np.array_equal(results[i], results[i + 2]) for i in range(4)) and int(tickets.abs().sum()) == 0
+
+
 def test_attention_in_storage_beyond_32_bits():
     """Pages whose values lie more than 2^32 bytes and 2^31 values from the entry's start."""
     from etalii.dllm_b200.cache.paged import KvView
