@@ -1504,6 +1504,8 @@ DLLM_EXPORT int dllm_attention_shared(const DllmAttentionShared* call, int bytes
     return DLLM_UNSUPPORTED_SIZE;
   Shape s = shape_of(dtype, heads, kv_heads, head_dim, groups, max_rows, max_context);
   if ((long long)groups * s.tiles > 65535) return DLLM_UNSUPPORTED_SIZE;
+  if (s.splits > s.cluster && (!c.scratch || !c.tickets)) return DLLM_BAD_ARGUMENT;
+  if (s.splits > s.cluster && ((uintptr_t)c.scratch & 15)) return DLLM_UNSUPPORTED_SIZE;  // (fours of floats go there)
   Args a{c.out, c.q, KvLayout{c.base, c.page_table, c.max_pages, c.page_size, kv_heads, head_dim}, c.slots, c.positions, c.cuts,
          c.shared, c.scratch, c.tickets, c.status, heads, c.window, s.tiles, s.splits, s.cluster, c.tokens, max_rows, c.scale};
   const long long pages = c.pages;

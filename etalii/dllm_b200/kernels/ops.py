@@ -2429,8 +2429,8 @@ def attention_shared(out: torch.Tensor, q: torch.Tensor, cache, heads: int, scal
     int32: slots, positions [tokens] (a token's row of the page table, its position; -1 sees nothing and gives zeros);
     groups [count + 1], the groups' first tokens (they follow one another); shared [count], how many pages from the first on
     are the same in the table rows of all of a group's tokens (more than there are: all). A group has at most `max_rows` tokens (more:
-    `raise_if_failed` says so) and positions lie below `max_context`. scratch, tickets: `attention_shared_scratch`; the
-    tickets are int32 zeros, left zero."""
+    `raise_if_failed` says so) and positions lie below `max_context`. scratch (aligned to 16 bytes), tickets:
+    `attention_shared_scratch`; the tickets are int32 zeros, left zero."""
     _cuda(out, q, slots, positions, groups, shared, scratch, tickets)
     count, tokens, width = groups.numel() - 1, q.shape[0], heads * cache.head_dim
     if not attention_shared_supported(cache):
@@ -2448,6 +2448,8 @@ def attention_shared(out: torch.Tensor, q: torch.Tensor, cache, heads: int, scal
     floats, words = attention_shared_scratch(cache, heads, max(count, 1), max_rows, max_context)
     if scratch.numel() < floats or tickets.numel() < words:
         raise KernelError(f"attention_shared: scratch of {scratch.numel()} floats and {tickets.numel()} tickets: {floats} and {words}")
+    if floats and scratch.data_ptr() % 16:
+        raise KernelError("attention_shared: scratch is not aligned to 16 bytes")
     if max_context > cache.max_pages * cache.page_size:
         raise KernelError(f"attention_shared: contexts of {max_context} in table rows of {cache.max_pages} pages")
     call = _ATTENTION_SHARED.pack(

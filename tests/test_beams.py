@@ -141,6 +141,21 @@ def test_the_list_refuses():
         CacheRows([(torch.zeros((1, 2, 64 * 1), dtype=torch.bfloat16), table, 1, 1, 0)], [], 64)
 
 
+@pytest.mark.parametrize("scratch,tickets,says", [(0x10008, 0x20000, "unsupported"), (0x10004, 0x20000, "unsupported"),
+                                                  (0, 0x20000, "argument"), (0x10000, 0, "argument")])
+@pytest.mark.parametrize("dtype,dim", [(0, 64), (1, 32), (1, 64)])
+def test_attention_over_shared_pages_refuses_its_scratch(scratch, tickets, says, dtype, dim):
+    """Two tokens on 9,000 positions, which several clusters share: the entry point looks at the scratch's address before it
+    launches anything. (The addresses are nobody's.)"""
+    from etalii.dllm_b200.kernels import ops
+
+    assert ops._shared_shape(dtype, 4, 2, dim, 1, 2, 9002)[0] > 0
+    call = ops._ATTENTION_SHARED.pack(*[0x1000 * (i + 1) for i in range(8)], scratch, tickets, 0x30000, 0, 200, 2, 141, 64, dtype, 4, 2, dim, 1,
+                                      2, 9002, 0, 0.1)
+    status = ops._fn("attention_shared", "dllm_attention_shared")(call, ops._ATTENTION_SHARED.size)
+    assert says in ops._STATUS[status]
+
+
 def test_plain_choice_by_hand():
     """Two beams, four tokens, token 3 ends a text: worked out on paper."""
     logits = np.log(np.array([[0.5, 0.3, 0.1, 0.1], [0.05, 0.05, 0.1, 0.8]]))

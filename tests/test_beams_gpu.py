@@ -601,6 +601,22 @@ def test_attention_refusals():
                                _i32(long.shared), 2, 9002, torch.zeros(scratch, device=DEV), torch.zeros(tickets, dtype=torch.int32, device=DEV))
 
 
+def test_attention_refuses_scratch_that_is_not_aligned():
+    from etalii.dllm_b200.cache.paged import KvView
+
+    o = ops()
+    for dtype, dim in ((torch.float32, 64), (torch.bfloat16, 32), (torch.bfloat16, 128)):
+        long = Pages("chunk", [(0, [9000, 9001])], 4, 2, dim, dtype)
+        view = KvView(long.storage.to(DEV), long.table.to(DEV), 64, 2, dim, None)
+        floats, words = o.attention_shared_scratch(view, 4, 1, 2, 9002)
+        q = long.q.to(DEV)
+        for offset in (1, 2, 3):
+            with pytest.raises(o.KernelError, match="aligned"):
+                o.attention_shared(torch.empty_like(q), q, view, 4, 0.1, 0, _i32(long.slots), _i32(long.positions), _i32(long.cuts),
+                                   _i32(long.shared), 2, 9002, torch.zeros(floats + 4, device=DEV)[offset:],
+                                   torch.zeros(words, dtype=torch.int32, device=DEV))
+
+
 # ---- whole searches --------------------------------------------------------------------------------------------------
 
 
