@@ -144,8 +144,9 @@ __global__ void __launch_bounds__(WARPS * 32) decode_attention_cluster_kernel(
     close_group();
   };
 
-  // this warp's first page: keys of earlier steps do not change any more, so it is copied before the wait on the
-  // projection kernel; the row that kernel writes (position end - 1) is read again after the wait
+  // this warp's first page: keys of earlier steps do not change any more (a kernel that moves them is over before any behind it
+  // starts: common.cuh), so it is copied before the wait on the projection kernel; the row that kernel writes (position end - 1)
+  // is read again after the wait
   int my_first = (int)rank * WARPS + warp;
   if (my_first < tiles) copy_page(key_of(my_first));
   // The tile that holds the newest key belongs to one warp of the cluster. That warp asks for the row right after

@@ -7,6 +7,7 @@
 // page's own number stays. States are copied whole. All beams of a sequence move at once, in place: a thread holds the
 // same 16 (or 4) bytes of all beams that move before it writes any of them, so any permutation and any fan-out is right and
 // no second buffer is needed. Beams that keep to themselves are neither read for their own sake nor written.
+// Attention kernels read page tables and cached rows ahead of their wait: the kernel behind this one starts when this one is over.
 //
 // The work is cut into pieces that a list on the device names, made once for a cache: 32 rows of a plane (one layer's keys or
 // values of one head) of the newest page, 8 KB of a state, a page table. A block moves one piece of one sequence's beams.
@@ -55,7 +56,6 @@ __global__ void __launch_bounds__(THREADS) reorder_kernel(const Piece* __restric
                                                           int length_stride, int ahead, int beams, int page_size) {
   __shared__ long long from[BEAMS];  // where a beam that moves comes from, 0 for one that stays
   __shared__ char* to[BEAMS];
-  pdl_launch_dependents();
   const int b = blockIdx.y;
   const Piece piece = pieces[blockIdx.x];
   pdl_wait();

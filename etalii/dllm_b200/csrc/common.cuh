@@ -30,6 +30,9 @@ static inline int dllm_launch_status() {
 // writes (weights, tables), and must call `pdl_wait` before it touches anything an earlier kernel produced and
 // before its own first write. Launched without the attribute both calls do nothing. DLLM_B200_PDL=0 turns the
 // attribute off.
+// Attention also reads positions, slots, page tables and the cached rows of earlier steps ahead of its wait. A kernel
+// that writes one of these other than as the step's own newest row (decode_advance, beam_reorder) therefore does not let its
+// dependents go early: they start when it is over.
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

@@ -2338,7 +2338,8 @@ def beam_select(parents: torch.Tensor, tokens: torch.Tensor, out: tuple, logits:
 def beam_reorder(rows, slots: torch.Tensor, parents: torch.Tensor, lengths: torch.Tensor, ahead: int = 0) -> None:
     """Beam i of sequence b takes over what beam parents[b, i] keeps, all beams at once, in place (csrc/beam_reorder.cu).
     `rows`: the cache's list (`cache.beams.CacheRows`); slots, parents int32 [sequences, beams]; lengths int32, one a
-    sequence or one a beam (then a sequence's first counts): the positions that its beams have cached, less `ahead`."""
+    sequence or one a beam (then a sequence's first counts): the positions that its beams have cached, less `ahead`. The next
+    kernel on the stream starts when the move is over (attention reads tables and rows ahead of its wait)."""
     _cuda(rows.pieces, slots, parents, lengths)
     sequences, beams = parents.shape
     if not 0 < beams <= MAX_BEAMS:

@@ -332,6 +332,50 @@ def test_move_refusals():
             o.beam_reorder(rows, slots, parents, lengths)
 
 
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float32, 64)])
+def test_move_is_over_before_the_attention_behind_it_reads(dtype, dim):
+    """Attention asks for positions, page tables and rows of earlier steps ahead of its wait: right behind a move, in one graph, it
+    gives what it gives when the move has long been over."""
+    from types import SimpleNamespace
+
+    from etalii.dllm_b200.cache.beams import CacheRows
+    from etalii.dllm_b200.cache.paged import KvView
+
+    o, beams, n, layers, kv_heads, length = ops(), 8, 3, 24, 4, 300
+    g = torch.Generator().manual_seed(dim)
+    count = n * beams
+    storage = torch.randn((layers, count * 6, 2, kv_heads, 64, dim), generator=g).to(dtype).to(DEV)
+    table = torch.randperm(count * 6, generator=g).to(torch.int32).view(count, 6).contiguous().to(DEV)
+    slots, parents = _i32(list(range(count))), _i32([[(i + 1) % beams for i in range(beams)]] * n)
+    q = (torch.randn((count, 2 * kv_heads * dim), generator=g) * 1.5).to(dtype).to(DEV)
+    rows = CacheRows([(storage, table, kv_heads, dim, dim)], [], 64)
+    view = KvView(storage[layers - 1], table, 64, kv_heads, dim, None)
+    batch = SimpleNamespace(tok_pos=_i32([length - 1] * count), tok_seq=_i32(list(range(count))), slots=slots, n_seqs=count, n_tokens=count,
+                            max_new=1, max_context=length, tile_seq=_i32([0]), tile_first=_i32([0]), cu_seqlens=_i32(list(range(count + 1))),
+                            n_tiles=0)
+    lengths = _i32([length] * n)
+
+    def attend(out):
+        kernel = o.attention_decode_cluster if dtype == torch.bfloat16 else o.attention_blocks
+        kernel(out, q, view, 2 * kv_heads, dim ** -0.5, 0, batch)
+
+    behind, alone = torch.empty_like(q), torch.empty_like(q)
+    attend(behind)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(3):
+            o.beam_reorder(rows, slots.view(n, beams), parents, lengths)
+            attend(behind)
+    for _ in range(20):
+        graph.replay()
+        torch.cuda.synchronize()
+        attend(alone)
+        torch.cuda.synchronize()
+        assert torch.equal(behind, alone)
+    o.raise_if_failed()
+
+
 # ---- attention over shared pages -------------------------------------------------------------------------------------
 
 

@@ -17,3 +17,22 @@ def test_blocks_that_read_each_others_memory_meet_in_order():
     code = _code("attention_shared.cu")
     assert "barrier.cluster.arrive" in code
     assert not re.search(r"barrier\.cluster\.arrive(?!\.release)", code) and not re.search(r"barrier\.cluster\.wait(?!\.acquire)", code)
+
+
+def _kernel(code, name):
+    """The body of the kernel `name`."""
+    at = code.index("{", re.search(rf"\b{name}\s*\(", code).end())
+    depth = 0
+    for i in range(at, len(code)):
+        depth += {"{": 1, "}": -1}.get(code[i], 0)
+        if depth == 0:
+            return code[at:i + 1]
+    raise AssertionError(f"{name} does not end")
+
+
+def test_what_attention_reads_ahead_of_its_wait_is_written_by_kernels_that_are_over():
+    """Attention reads positions, page tables and cached rows of earlier steps ahead of its wait. The kernels that write them
+    wait for the one in front and do not let the one behind start early."""
+    for source, kernel in (("beam_reorder.cu", "reorder_kernel"), ("elementwise.cu", "decode_advance_kernel")):
+        body = _kernel(_code(source), kernel)
+        assert "pdl_wait()" in body and "launch_dependents" not in body, (source, kernel)
