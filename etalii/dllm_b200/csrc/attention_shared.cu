@@ -1235,7 +1235,8 @@ __global__ void __launch_bounds__(FMA_THREADS) fma_kernel(const Args a) {
   __shared__ Plan p;
   __shared__ Stretch list;
   __shared__ __align__(16) float sm_p[PAGE * FMA_LD];
-  __shared__ float sm_max[2][2][FMA_ROWS], sm_fade[FMA_ROWS], sm_l[2][FMA_ROWS];
+  __shared__ float sm_max[2][2][FMA_ROWS], sm_l[2][FMA_ROWS];
+  __shared__ __align__(16) float sm_fade[FMA_ROWS];  // (read by fours)
   __shared__ float2 sm_ml[FMA_ROWS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int hd = a.cache.head_dim, kv = blockIdx.y, per_kv = a.heads / a.cache.kv_heads;

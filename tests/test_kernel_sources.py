@@ -36,3 +36,15 @@ def test_what_attention_reads_ahead_of_its_wait_is_written_by_kernels_that_are_o
     for source, kernel in (("beam_reorder.cu", "reorder_kernel"), ("elementwise.cu", "decode_advance_kernel")):
         body = _kernel(_code(source), kernel)
         assert "pdl_wait()" in body and "launch_dependents" not in body, (source, kernel)
+
+
+def test_shared_arrays_that_are_read_in_16_bytes_are_aligned_to_them():
+    """attention_shared: an array of floats in shared memory has no alignment but a float's unless it is given one."""
+    code = _code("attention_shared.cu")
+    read = set(re.findall(r"\bfour\((sm_\w+)", code))
+    read |= set(re.findall(r"reinterpret_cast<(?:const )?(?:float4|ulonglong2|uint4)\s*\*>\(\s*&?\s*(sm_\w+)", code))
+    assert {"sm_fade", "sm_shift", "sm_p"} <= read
+    declarations = re.findall(r"__shared__ ([^;]*);", code)
+    for name in read:
+        holding = [d for d in declarations if re.search(rf"\b{name}\s*\[", d)]
+        assert holding and all("__align__(16)" in d for d in holding), name
