@@ -21,6 +21,7 @@ from ..sampling.sampler import Sampler
 from ..weights.loader import load_weights
 from ..weights.random_init import random_tensors
 from ..sampling.beams import BeamOptions
+from ..parts.attention import SHARED_FROM_CONTEXT
 from .batch import BatchBuffers
 from .beam import BeamGraph, BeamResult, SharedRows, plan_beam_batches, search_batch
 from .decode import DecodeGraph
@@ -64,7 +65,7 @@ class Engine:
         `decode_logits`: decode runs always compute the logits (they stay readable in the run's buffer); by default
         a greedy run lets the head product choose the token itself and stores no logits. `split_chunks`: steps in which
         sequences bring at most this many new tokens (and one of them more than one) cut their contexts' keys over the
-        device (`ops.attention_shared`), where the parts can and contexts are long enough to gain. 0: never."""
+        device (`ops.attention_shared`), where the parts can and a context is long enough to gain (768 positions). 0: never."""
         if not torch.cuda.is_available():
             raise RuntimeError("no CUDA device: this library has no CPU path")
         self.config = config
@@ -144,7 +145,7 @@ class Engine:
             starts.append(self.cache.length(slot))
         self.cache.sync_tables()
         batch = self.buffers.fill(slots, new_tokens, starts, want)
-        if 1 < batch.max_new <= self.split_chunks:
+        if 1 < batch.max_new <= self.split_chunks and batch.max_context >= SHARED_FROM_CONTEXT:
             batch.shared = self._shared_rows(batch)
         logits = self.model.forward(batch)
         for slot, tokens in zip(slots, new_tokens):

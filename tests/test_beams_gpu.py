@@ -826,6 +826,29 @@ def test_short_chunks_over_the_whole_device(dtype, tolerance):
     assert rel_error(outs[1], outs[0]) <= tolerance
 
 
+def test_short_chunks_of_short_contexts_are_steps_like_any_other():
+    """An engine that splits chunks runs a step below 768 positions as one that does not: from the launcher of all layers where
+    there is one, to the same bits."""
+    config, _ = model_case("a")
+    config = {**config, "num_attention_heads": 4, "num_key_value_heads": 2, "head_dim": 64, "hidden_size": 128,
+              "intermediate_size": 320, "max_position_embeddings": 1024}
+    weights = P.random_weights(config, 5, std=0.05)
+    prompts = prompts_for(config, [700] + [90] * 8)
+    outs = []
+    for n in (0, 8):
+        engine = make_engine(config, weights, "bfloat16", max_tokens=8192, max_length=1024, split_chunks=n)
+        launched, run = [], engine.model.native_layers.run
+        engine.model.native_layers.run = lambda *a, launched=launched, run=run: (launched.append(1), run(*a))
+        slots = engine.open(9)
+        engine.step(slots, prompts)
+        outs.append(host(engine.step(slots, [p[:8] for p in prompts])))   # 72 tokens on at most 708 positions
+        assert len(launched) == 2 and getattr(engine.last_batch, "shared", None) is None
+        engine.step(slots, [p[:60] for p in prompts])
+        host(engine.step(slots, [p[:8] for p in prompts]))                # on 776
+        assert len(launched) == (4 if n == 0 else 3) and (getattr(engine.last_batch, "shared", None) is not None) == (n > 0)
+    assert np.array_equal(*outs)
+
+
 def test_the_command_line(tmp_path):
     from etalii.dllm_b200.weights.random_init import write_model
 
