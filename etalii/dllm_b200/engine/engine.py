@@ -156,9 +156,9 @@ class Engine:
 
     def _shared_rows(self, batch) -> SharedRows:
         """Every sequence's new tokens as a group of `ops.attention_shared`: all pages in common."""
-        packed = [slot for slot, count in zip(batch.h_slots, batch.h_new) for _ in range(count)]
-        both = torch.tensor(packed + [self.cache.max_pages] * batch.n_seqs, dtype=torch.int32, device=self.rt.device)
-        return SharedRows(both[:len(packed)], batch.cu_seqlens, both[len(packed):], batch.max_new)
+        slots = batch.slots.index_select(0, batch.tok_seq)  # (on the device: nothing waits)
+        shared = torch.full((batch.n_seqs,), self.cache.max_pages, dtype=torch.int32, device=self.rt.device)
+        return SharedRows(slots, batch.cu_seqlens, shared, batch.max_new)
 
     def check(self) -> None:
         """Raises `KernelError` if a kernel of a step that has finished reported that its results are invalid."""

@@ -849,6 +849,25 @@ def test_short_chunks_of_short_contexts_are_steps_like_any_other():
     assert np.array_equal(*outs)
 
 
+def test_short_chunks_over_the_whole_device_wait_for_nothing():
+    """What a step tells the attention over shared pages is made on the device, behind what is running there."""
+    config, weights = model_case("a")
+    config = {**config, "max_position_embeddings": 1024}
+    engine = make_engine(config, P.random_weights(config, 5, std=0.05), "float32", max_tokens=8192, max_length=1024, split_chunks=4)
+    slots = engine.open(3)
+    engine.step(slots, prompts_for(config, [800, 70, 5]))
+    engine.step(slots, [[1, 2, 3], [4], [5, 6, 7, 8]])
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        shared = engine._shared_rows(engine.last_batch)
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    assert shared.slots.tolist() == [slots[0]] * 3 + [slots[1]] + [slots[2]] * 4 and shared.slots.dtype == torch.int32
+    assert shared.shared.tolist() == [engine.cache.max_pages] * 3 and shared.max_rows == 4
+    assert shared.groups.tolist() == [0, 3, 4, 8]
+
+
 def test_the_command_line(tmp_path):
     from etalii.dllm_b200.weights.random_init import write_model
 
