@@ -308,6 +308,7 @@ class Engine:
         if max_new_tokens <= 0:
             return [[BeamResult((), 0.0, len(p), "length")] for p in prompts]
         limits = [min(int(max_new_tokens), window - len(p)) for p in prompts]
+        options.check_length(max(limits, default=0))
         batches = plan_beam_batches([len(p) for p in prompts], limits, options.beams, self.cache.page_size,
                                     self.cache.smallest_pool(), self.cache.n_slots, max_batch)
         out: list[list[BeamResult] | None] = [None] * len(prompts)

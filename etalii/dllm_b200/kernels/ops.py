@@ -2306,6 +2306,8 @@ def beam_select(parents: torch.Tensor, tokens: torch.Tensor, out: tuple, logits:
     stops = stop_ids.numel() if stop_ids is not None else 0
     if stops > MAX_BEAM_STOPS:
         raise KernelError(f"beam_select: {stops} stop tokens: at most {MAX_BEAM_STOPS}")
+    if not abs(length_penalty) < 3.4e38:  # (also refuses NaN)
+        raise KernelError(f"beam_select: length_penalty {length_penalty}")
     f32, i32 = torch.float32, torch.int32
     if not (logits.dtype is f32 and scores.dtype is f32 and finished.dtype is f32 and scores_out.dtype is f32
             and finished_out.dtype is f32 and scratch.dtype is f32 and parents.dtype is i32 and tokens.dtype is i32

@@ -21,6 +21,23 @@ def test_options_refuse(wrong):
         BeamOptions(**wrong)
 
 
+@pytest.mark.parametrize("penalty", [math.inf, -math.inf, 1e400])
+def test_options_refuse_a_penalty_that_is_no_number(penalty):
+    with pytest.raises(ValueError, match="finite"):
+        BeamOptions(length_penalty=penalty)
+
+
+@pytest.mark.parametrize("tokens,largest", [(1, 96.0), (2047, 96 / 11), (65535, 6.0)])
+def test_options_refuse_a_penalty_that_leaves_no_score(tokens, largest):
+    BeamOptions(length_penalty=largest * 0.999).check_length(tokens)
+    for penalty in (largest * 1.001, 1e300):
+        with pytest.raises(ValueError, match="2 \\*\\* 96"):
+            BeamOptions(length_penalty=penalty).check_length(tokens)
+    BeamOptions(length_penalty=1e300).check_length(0)
+    # at the bound the least log probability that a token can have (1 - 2^-24 as a probability) is still a normal float32
+    assert np.float32(2.0 ** -24) / np.float32(2.0 ** 96) >= np.finfo(np.float32).tiny
+
+
 def test_options_defaults():
     assert (BeamOptions().beams, BeamOptions().length_penalty, BeamOptions().early_stopping) == (4, 1.0, False)
 

@@ -805,6 +805,29 @@ def test_search_in_batches_and_its_limits():
     assert engine.generate(prompts[:1], 4, ignore_eos=True)[0].tokens  # the engine goes on as before
 
 
+@pytest.mark.parametrize("penalty", [20.0, 1e30, 1e300])
+def test_search_refuses_a_penalty_that_leaves_no_score(penalty):
+    """(tokens) ** penalty beyond float32 would give every text that has ended the score -0, or raise in the middle of a search."""
+    from etalii.dllm_b200.sampling.beams import BeamOptions
+
+    config, weights = model_case("a")
+    engine = make_engine(config, weights, "float32")
+    prompts = prompts_for(config, [5, 9])
+    with pytest.raises(ValueError, match="length_penalty"):
+        engine.beam_search(prompts, 40, BeamOptions(beams=2, length_penalty=penalty), stop_token_ids=range(0, 8), ignore_eos=True)
+    assert engine.cache.slots.held == 0
+    found = engine.beam_search(prompts, 40, BeamOptions(beams=2, length_penalty=8.0), ignore_eos=True)
+    assert all(np.isfinite(text.score) and text.score < 0 for texts in found for text in texts)
+
+
+@pytest.mark.parametrize("penalty", [math.inf, math.nan, 1e300])
+def test_choice_refuses_a_penalty_that_is_no_float32(penalty):
+    case = Choice(1, 2, 2, 50, seed=0)
+    case.run()
+    with pytest.raises(ops().KernelError, match="length_penalty"):
+        case.run(penalty=penalty)
+
+
 @pytest.mark.parametrize("dtype,tolerance", [("float32", 2e-5), ("bfloat16", 2e-2)])
 def test_short_chunks_over_the_whole_device(dtype, tolerance):
     """Steps of a few tokens each, keys cut over the device: the logits of the engine that walks them."""
