@@ -173,6 +173,53 @@ def test_attention_over_shared_pages_refuses_its_scratch(scratch, tickets, says,
     assert says in ops._STATUS[status]
 
 
+def _step(tokens, context, groups=1, decode=True, shared=True):
+    from types import SimpleNamespace
+
+    from etalii.dllm_b200.engine.beam import SharedRows
+
+    cuts = torch.zeros(groups + 1, dtype=torch.int32)
+    batch = SimpleNamespace(is_decode=decode, n_tokens=tokens, max_context=context)
+    if shared:
+        batch.shared = SharedRows(None, cuts, None, tokens // groups)
+    return batch
+
+
+def _entry(kv_heads, dim, dtype, value_dim=0, keys_only=False, page=64):
+    from etalii.dllm_b200.cache.paged import KvView
+
+    return KvView(torch.zeros(1, dtype=dtype), torch.zeros((1, 4), dtype=torch.int32), page, kv_heads, dim, None, value_dim, keys_only)
+
+
+@pytest.mark.parametrize("kv_heads,dim,dtype,tokens,groups,least", [
+    (3, 64, torch.bfloat16, 64, 8, (128 << 20) / (64 * 768)), (3, 64, torch.bfloat16, 4, 1, (128 << 20) / (4 * 768)),
+    (8, 128, torch.bfloat16, 64, 8, (64 << 20) / (64 * 4096)),   # (eight prompts of eight kv heads: a MB each)
+    (8, 128, torch.bfloat16, 8, 1, (32 << 20) / (8 * 4096)), (32, 64, torch.bfloat16, 32, 8, (256 << 20) / (32 * 8192)),
+    (3, 64, torch.float32, 64, 8, (64 << 20) / (64 * 1536)), (8, 128, torch.float32, 8, 1, (64 << 20) / (8 * 8192))])
+def test_from_which_contexts_on_beams_read_shared_pages(kv_heads, dim, dtype, tokens, groups, least):
+    """By the bytes of keys and values counted for every beam."""
+    from etalii.dllm_b200.parts.attention import reads_shared_pages
+
+    cache = _entry(kv_heads, dim, dtype)
+    first = math.ceil(least)
+    assert reads_shared_pages(_step(tokens, first, groups), cache) and not reads_shared_pages(_step(tokens, first - 1, groups), cache)
+    assert not reads_shared_pages(_step(tokens, 1 << 30, groups, shared=False), cache)
+
+
+def test_what_else_decides_whether_a_step_reads_shared_pages():
+    from etalii.dllm_b200.parts.attention import reads_shared_pages
+
+    for dtype in (torch.float32, torch.bfloat16):
+        cache = _entry(2, 64, dtype)  # a few tokens appended: by the longest context
+        assert reads_shared_pages(_step(2, 768, decode=False), cache) and not reads_shared_pages(_step(2, 767, decode=False), cache)
+        for other in (_entry(2, 60, dtype), _entry(2, 264, dtype), _entry(2, 64, dtype, value_dim=32), _entry(2, 64, dtype, keys_only=True),
+                      _entry(2, 64, dtype, page=32)):
+            assert not reads_shared_pages(_step(64, 1 << 20, 8), other)
+    assert not reads_shared_pages(_step(64, 1 << 20, 8), _entry(2, 64, torch.float16))
+    # bfloat16 heads that the cluster kernel of single tokens does not take
+    assert reads_shared_pages(_step(4, 10), _entry(2, 72, torch.bfloat16)) and not reads_shared_pages(_step(4, 10), _entry(2, 80, torch.bfloat16))
+
+
 def test_plain_choice_by_hand():
     """Two beams, four tokens, token 3 ends a text: worked out on paper."""
     logits = np.log(np.array([[0.5, 0.3, 0.1, 0.1], [0.05, 0.05, 0.1, 0.8]]))

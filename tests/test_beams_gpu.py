@@ -719,6 +719,62 @@ def test_search_whose_beams_read_shared_pages(dtype, head_dim, monkeypatch):
         assert abs(one[0].score - other[0].score) <= (1e-3 if dtype == "float32" else 0.06)
 
 
+@pytest.fixture
+def calls(monkeypatch):
+    """How often each attention operator of single tokens has been called."""
+    module, count = ops(), {}
+    for name in ("attention_shared", "attention_decode_cluster", "attention_decode", "attention_blocks"):
+        def counted(*a, name=name, inner=getattr(module, name), **k):
+            count[name] = count.get(name, 0) + 1
+            return inner(*a, **k)
+
+        monkeypatch.setattr(module, name, counted)
+    return count
+
+
+@pytest.mark.parametrize("beams,taken,left", [(8, "attention_shared", "attention_decode_cluster"),
+                                              (4, "attention_decode_cluster", "attention_shared")])
+def test_search_reads_shared_pages_where_the_rule_says_so(beams, taken, left, calls):
+    """8 kv heads of 128, contexts of up to 1,024: eight beams are 32 MB of keys and values a layer, four are 16."""
+    from etalii.dllm_b200.sampling.beams import BeamOptions
+
+    config, _ = model_case("a")
+    config = {**config, "num_attention_heads": 16, "num_key_value_heads": 8, "head_dim": 128, "max_position_embeddings": 1024}
+    engine = make_engine(config, P.random_weights(config, 6, std=0.08), "bfloat16", max_tokens=8192, max_length=1024)
+    found = engine.beam_search(prompts_for(config, [200]), 20, BeamOptions(beams=beams), ignore_eos=True)
+    assert calls.get(taken, 0) > 0 and calls.get(left, 0) == 0 and len(found[0]) == beams
+
+
+@pytest.mark.parametrize("dtype,head_dim,other", [("float32", 64, "attention_blocks"), ("bfloat16", 64, "attention_decode_cluster"),
+                                                  ("bfloat16", 128, "attention_decode_cluster")])
+def test_search_finds_the_same_by_either_attention(dtype, head_dim, other, calls, monkeypatch):
+    """The rule moved to either side: the operator that it names runs and the other does not; float32 finds the same texts."""
+    from etalii.dllm_b200.parts import attention
+    from etalii.dllm_b200.sampling.beams import BeamOptions
+
+    config, _ = model_case("a")
+    config = {**config, "num_attention_heads": 4, "num_key_value_heads": 2, "head_dim": head_dim, "max_position_embeddings": 512}
+    weights = P.random_weights(config, 6, std=0.08)
+    prompts = prompts_for(config, [20, 128, 200])
+    reads, found = attention.reads_shared_pages, []
+    for shared in (True, False):
+        monkeypatch.setattr(attention, "SHARED_FROM_BYTES", {d: (0, 0) if shared else (1 << 60, 1 << 60) for d in attention.SHARED_FROM_BYTES})
+        # (the MB for each prompt and kv head is the rule's too: a step that counts as many positions as that takes)
+        monkeypatch.setattr(attention, "reads_shared_pages", lambda batch, cache: reads(
+            type("Step", (), {**vars(batch), "max_context": 1 << 24}), cache) if getattr(batch, "shared", None) is not None else False)
+        engine = make_engine(config, weights, dtype, max_tokens=4096)
+        calls.clear()
+        found.append(engine.beam_search(prompts, 40, BeamOptions(beams=3), ignore_eos=True))
+        ran, kept = ("attention_shared", other) if shared else (other, "attention_shared")
+        decoded = calls.get(ran, 0) - (config["num_hidden_layers"] if ran == "attention_blocks" else 0)  # (the prompt's step)
+        assert decoded > 0
+        assert calls.get(kept, 0) == (config["num_hidden_layers"] if kept == "attention_blocks" else 0)
+    for one, two in zip(*found):
+        if dtype == "float32":
+            assert [r.tokens for r in one] == [r.tokens for r in two]
+        assert abs(one[0].score - two[0].score) <= (1e-3 if dtype == "float32" else 0.06)
+
+
 def test_one_beam_is_the_greedy_choice():
     from etalii.dllm_b200.sampling.beams import BeamOptions
 
