@@ -658,7 +658,7 @@ DLLM_EXPORT int dllm_beam_select(const DllmBeamSelect* call, int bytes) {
   const DllmBeamSelect& c = *call;
   const int sequences = c.sequences, beams_in = c.beams_in, beams = c.beams, vocab = c.vocab, n_stops = c.n_stops;
   if (sequences <= 0) return DLLM_OK;
-  if (beams_in <= 0 || beams <= 0 || vocab <= 0 || n_stops < 0 || (n_stops > 0 && !c.stop_ids) || c.row_stride < vocab)
+  if (beams_in <= 0 || beams <= 0 || vocab <= 0 || n_stops < 0 || (n_stops > 0 && !c.stop_ids) || c.row_stride < vocab || !c.produced)
     return DLLM_BAD_ARGUMENT;
   if (beams_in > MAX_BEAMS || beams > MAX_BEAMS || n_stops > MAX_STOPS || (long long)sequences * beams_in > 65535)
     return DLLM_UNSUPPORTED_SIZE;

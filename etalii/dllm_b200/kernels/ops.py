@@ -1674,7 +1674,8 @@ def _status_word() -> torch.Tensor:
 def raise_if_failed() -> None:
     """Raises if a kernel has set the status word since the last look: a bounded wait on an mbarrier ran out
     (codes 2-5 the tile product, 12-21 the tcgen05 attention, 32-33 the product that streams through shared memory, 42-45
-    the experts' tile products), a token saw more keys than its step was prepared for (50), a group had more tokens (51),
+    the experts' tile products, 52-55 the tcgen05 attention over shared pages), a token saw more keys than its step was
+    prepared for (50), a group had more tokens (51),
     or the embedding met a token outside its table (64). Results computed since are not valid. The word lives in
     pinned host memory, so the look costs no synchronisation; it is meaningful after the host has waited for the
     kernels in question (a `.tolist()`, a copy to the host, a synchronize)."""
@@ -2288,8 +2289,8 @@ def beam_select(parents: torch.Tensor, tokens: torch.Tensor, out: tuple, logits:
     [sequences, beams] in descending order, -inf where there is none, finished_at int32 [sequences, beams, 2], done int32
     [sequences]); `out`: the same four for the next step, scores [sequences, beams] (the same tensors where the shapes
     allow). parents, tokens int32 [sequences, beams]: the beam (of the sequence's) that each place continues, and with which
-    token. A place without a beam has score -inf, itself as parent and token 0. finished_at: (tokens produced before the
-    stop token, the beam that it followed).
+    token. A place without a beam has score -inf, itself as parent (the last of beams_in where there is no such beam) and
+    token 0. finished_at: (tokens produced before the stop token, the beam that it followed).
     The beams have produced[0] + steps[0] tokens (int32, `steps` may be None); while those are fewer than `min_tokens` a
     stop token (`stop_ids` int32, at most MAX_BEAM_STOPS) ends nothing, and it is never a beam's next token. `history`
     int32 [capacity, sequences, beams]: the parents are kept at history[steps[0]] too. scratch: `beam_select_scratch`
@@ -2320,6 +2321,8 @@ def beam_select(parents: torch.Tensor, tokens: torch.Tensor, out: tuple, logits:
             and done.numel() == done_out.numel() == sequences and tickets.numel() >= sequences):
         raise KernelError(f"beam_select: logits {tuple(logits.shape)}, scores {tuple(scores.shape)} and {beams} beams do not "
                           f"go together with the shapes of the rest")
+    if not produced.numel() or (steps is not None and not steps.numel()):
+        raise KernelError("beam_select: produced and steps hold a number each")
     at = scratch.data_ptr()
     if scratch.numel() < rows * _beam_select_parts(rows, vocab) * (2 + 2 * beams) or at % 8:
         raise KernelError("beam_select: scratch is too small (beam_select_scratch) or not aligned to 8 bytes")

@@ -173,6 +173,15 @@ def test_attention_over_shared_pages_refuses_its_scratch(scratch, tickets, says,
     assert says in ops._STATUS[status]
 
 
+def test_choice_refuses_to_go_without_a_step_number():
+    """A null address where the number of tokens so far is read. (The other addresses are nobody's: nothing is launched.)"""
+    from etalii.dllm_b200.kernels import ops
+
+    at = [0x1000 * (i + 1) for i in range(17)]
+    call = ops._BEAM_SELECT.pack(at[0], 50, at[1], at[2], at[3], at[4], 0, 0, 0, *at[5:11], 0, at[11], at[12], 0, 0, 0, 1, 4, 4, 50, 0, 0, 1.0)
+    assert ops._STATUS[ops._fn("beam_select", "dllm_beam_select")(call, ops._BEAM_SELECT.size)] == "bad argument"
+
+
 def _step(tokens, context, groups=1, decode=True, shared=True):
     from types import SimpleNamespace
 

@@ -243,6 +243,18 @@ def test_choice_refusals():
         o.beam_select_scratch(0, 4, 50, 4)
 
 
+def test_choice_refuses_numbers_that_are_not_there():
+    case = Choice(1, 2, 2, 50, seed=0)
+    case.run(steps=_i32([0]))
+    with pytest.raises(ops().KernelError, match="number each"):
+        case.run(steps=_i32([]))
+    state = tuple(t.to(DEV) for t in (case.scores, case.finished, case.finished_at, case.done))
+    out = torch.zeros((1, 2), dtype=torch.int32, device=DEV)
+    with pytest.raises(ops().KernelError, match="number each"):
+        ops().beam_select(out, out.clone(), state, case.logits.to(DEV), state, _i32([]), torch.zeros(ops().beam_select_scratch(1, 2, 50, 2), device=DEV),
+                          _i32([0]))
+
+
 # ---- the move --------------------------------------------------------------------------------------------------------
 
 
