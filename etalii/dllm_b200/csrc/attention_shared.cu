@@ -14,8 +14,9 @@
 // nobody waits) joins them in order.
 //
 // bfloat16, head sizes that are multiples of 16: from 64 to 128 on the 5th-generation tensor cores (namespace t5), below
-// with mma.sync (mma_kernel). Probabilities are rounded to bfloat16 as the second product's operand. Everything else
-// (float32, other head sizes): fused multiply-adds on pages in shared memory (fma_kernel).
+// with mma.sync (mma_kernel). Probabilities are rounded to bfloat16 there, since both operands of the second product have the
+// values' type: results are 0.0019 to 0.0021 (relative, root mean square) from 64 bits, where only their own rounding would leave
+// 0.0017. Everything else (float32, other head sizes): fused multiply-adds on pages in shared memory (fma_kernel).
 //
 // A masked key has weight 0 by selection, not by arithmetic, and its value is not multiplied: a NaN or infinity in a place
 // that a token does not see leaves it alone. (Products on the tensor cores multiply zeros too: pages that some row
@@ -413,8 +414,8 @@ template <int HD> __device__ __forceinline__ int place(int r, int c) {
   return r * HD + 8 * (HD >= 64 ? c ^ (r & 7) : c ^ ((r >> 1) & 3));
 }
 
-// Heads of 16, 32 and 48. Bound by the chain from the plan to the join: 9 heads on 3 of 32, 1 x 4 beams on 100 positions 7.3 us, 8 x 4
-// on 1,000 9.8.
+// Heads of 16, 32 and 48. Bound by the chain from the plan to the join: 9 heads on 3 of 32, 1 x 4 beams on 110 positions 7.2 us, 8 x 4
+// on 1,020 10.7.
 // HD: the head size, padded (32, 64). A warp has 16 * MT query rows; WM warps (of 4) lie one above another in the tile.
 template <int HD, int MT, int WM, int STAGES>
 __global__ void __launch_bounds__(WM * 128) mma_kernel(const Args a) {
@@ -735,9 +736,9 @@ int launch_clusters(Kernel kernel, dim3 grid, int threads, size_t smem, int clus
 // Pages that some row sees in part are looked at: a value that is not finite is kept out of the product; such a step is added
 // by the softmax warps, key by key.
 // Every wait is bounded; a role that gives up sets the status word and leaves.
-// Bound by HBM where pages are many: two chunks of eight tokens on 40,000 positions, 32 heads on 8 of 128, 57.5 us (287 MB, 5.0 TB/s, 128
-// blocks); by the chain lookup, page, scores, softmax, outputs, join where they are few: 8 x 8 beams on 2,000 positions 26.3 us (77 MB,
-// two blocks a pair of prompt and kv head), 1 x 4 on 100, 9 heads on 3 of 64, 9.0 us, of which 2 are the plan, 2 the first page, 3 the join.
+// Bound by HBM where pages are many: two chunks of eight tokens on 40,000 positions, 32 heads on 8 of 128, 56.3 us (287 MB, 5.1 TB/s, 128
+// blocks); by the chain lookup, page, scores, softmax, outputs, join where they are few: 8 x 8 beams on 2,150 positions 26.3 us (77 MB,
+// two blocks a pair of prompt and kv head), 1 x 4 on 110, 9 heads on 3 of 64, 8.8 us, of which 2 are the plan, 2 the first page, 3 the join.
 namespace t5 {
 using namespace tc5;
 constexpr int KEYS = 2 * PAGE;
@@ -1214,7 +1215,7 @@ int launch(const Args& a, long long pages, dim3 grid, cudaStream_t stream) {
 // a page's 64 keys and four rows. The rows' maxima go through shared memory, the weights of a key's 16 rows lie side by side in
 // it. Sums: a thread has four dimensions and four rows, and every n-th key; the n groups are added at the end.
 // Bound by a page's chain (scores 1.0 us, maxima 0.4, weights 0.3, sums 0.9 for heads of 64 in float32: shared-memory reads and their
-// latency with eight warps): 9 heads on 3 of 64, 2 x 5 beams on 700 positions 14.9 us, 8 x 8 on 1,000 30. Half the instructions did
+// latency with eight warps): 9 heads on 3 of 64, 2 x 5 beams on 770 positions 14.2 us, 8 x 8 on 1,070 30. Half the instructions did
 // not shorten it (packed multiply-adds, four keys a thread with the dimensions over four lanes, redux: 17.1 us where it was 17.0).
 constexpr int FMA_ROWS = 16, FMA_THREADS = 256, FMA_DIM = 256, FMA_LD = 20;
 constexpr int FMA_MOST = 152 << 10;  // bytes of dynamic shared memory: heads of 128 in float32, two stages; of 256, one

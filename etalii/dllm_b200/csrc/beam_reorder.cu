@@ -13,7 +13,8 @@
 // values of one head) of the newest page, 8 KB of a state, a page table. A block moves one piece of one sequence's beams.
 // Bound by HBM: what is continued is read once, what moves is written once. Measured with 8, 16, 32 and 64 rows a piece, us: 8 x 8 beams of
 // 32 layers of 8 heads of 128, five of eight move, 44 rows 78.4, 65.3, 61.9, 62.0 (5.9 TB/s); 3 x 5 float32 beams in a ring, 30 layers
-// of 3 heads of 64, 61 rows 20.9, 19.7, 20.2, 21.9; with 8, 16 and 32 KB of a state a piece, 4 x 4 beams with 12 states of 1 MB 34.1,
+// of 3 heads of 64, 61 rows 20.9, 19.7, 20.2, 21.9 (1,083 blocks of 32 rows where 740 are resident: five of a multiprocessor, by registers;
+// 21.0 since the next move no longer starts under this one); with 8, 16 and 32 KB of a state a piece, 4 x 4 beams with 12 states of 1 MB 34.1,
 // 34.9, 36.2 (6.0 TB/s).
 #include "common.cuh"
 

@@ -42,7 +42,7 @@ def reads_shared_pages(batch, cache) -> bool:
     """Whether a step whose tokens share pages (`batch.shared`) attends with `ops.attention_shared`: it costs 9 to 12 µs
     whatever the contexts are, where the kernels that read every token's pages cost 3 to 10 µs and then grow with them. Beams: from
     so many bytes of keys and values on, counted for every beam (heads up to 64, above; and 1 MB for every prompt and kv head: their
-    blocks take turns). Short chunks: from 768 positions on. Measured, µs, shared and not: 8 x 8 beams, 9 heads on 3 of 64,
+    blocks take turns). A captured step counts the contexts that it may serve, so up to 1,024 positions more than there are. Short chunks: from 768 positions on. Measured, µs, shared and not: 8 x 8 beams, 9 heads on 3 of 64,
     1,000 positions 11.8 and 8.7, 4,000 15.0 and 20.4; 32 heads on 8 of 128, 500 positions 15.9 and 28.0, 4,000 32.4 and 102.5; 1 x 4, 2,000
     positions 13.1 and 9.6, 4,000 15.2 and 15.6; 32 heads on 32 of 64, 8 x 4 on 500 19.5 and 20.2, on 1,000 26.6 and 31.2; float32, 9 heads
     on 3 of 64, 8 x 8 beams on 250 positions 20.8 and 17.8, on 2,000 41.3 and 106.8; eight new tokens on 250, 1,000 and 16,000 positions, 32
