@@ -22,8 +22,8 @@
 //      what is before it. A list that does not hold them all (many equal logits) is given up for `beams` passes over the stretch.
 //   2. The block that finishes last for its sequence (a ticket counter; nobody waits) joins the stretches' sums,
 //      makes the totals and chooses among the stretches' lists the same way; a warp deals out places and pool.
-// Bound by HBM where the rows are many, by the latency of the two steps where they are few: 1 x 4 beams of 49,152 logits 7.9 us (2.5 to the
-// stretch's best, 1 for the ticket, 4 for the join), 8 x 8 of 128,256 17.3, 32 x 16 54.6 (230 MB of living rows, 4.2 TB/s; 6.3 while all
+// Bound by HBM where the rows are many, by the latency of the two steps where they are few: 1 x 4 beams of 49,152 logits 8.1 us (2.5 to the
+// stretch's best, 1 for the ticket, 4 for the join), 8 x 8 of 128,256 18.5, 32 x 16 54.9 (230 MB of living rows, 4.2 TB/s; 6.3 while all
 // multiprocessors have as many blocks, but 448 living rows are four for some and three for others). Blocks of a stretch that fits
 // their registers (4,096 of them for 512 rows of 128,256 instead of 512) spent most of their time on what a block costs. The next tile
 // by bulk copies into shared memory while this one is worked on changed nothing (8 x 8 18.0 us where it was 18.7, 32 x 16 57.1 where it was 55.4).
